@@ -63,6 +63,17 @@ class Tail(ctypes.Structure):
     ]
 
 
+class Rotary(ctypes.Structure):
+    _fields_ = [
+        ("cos", ctypes.c_void_p), ("cos_strides", _I64x3),
+        ("sin", ctypes.c_void_p), ("sin_strides", _I64x3),
+        ("dtype", ctypes.c_int32), ("R", ctypes.c_int32),
+        ("q", ctypes.c_void_p), ("q_strides", _I64x4),
+        ("q_out", ctypes.c_void_p), ("qo_strides", _I64x4),
+        ("H_q", ctypes.c_int32),
+    ]
+
+
 class Prefill(ctypes.Structure):
     _fields_ = [
         ("q", ctypes.c_void_p), ("q_strides", _I64x4),
@@ -118,6 +129,15 @@ SIGNATURES = {
                                             _P, _I64P, _I, _I, _P]),
     "fq_int8_cache_append": (ctypes.c_int, [ctypes.POINTER(Int4Cache), _I, _P, _I64P, _P, _I64P, _I, _P, _I64P,
                                             _P, _I64P, _I, _I, _P]),
+    "fq_int4_cache_append_rotated": (ctypes.c_int, [ctypes.POINTER(Int4Cache), _I, _P, _I64P, _P, _I64P, _I, _P,
+                                                    _I64P, _P, _I64P, _I, _I, ctypes.POINTER(Rotary), _P]),
+    "fq_int8_cache_append_rotated": (ctypes.c_int, [ctypes.POINTER(Int4Cache), _I, _P, _I64P, _P, _I64P, _I, _P,
+                                                    _I64P, _P, _I64P, _I, _I, ctypes.POINTER(Rotary), _P]),
+    "fq_rotate": (ctypes.c_int, [ctypes.POINTER(Rotary), _P, _I64P, _P, _I64P, _I, _I, _I, _I, _I, _P]),
+    "fq_dequant_int4": (ctypes.c_int, [ctypes.POINTER(Int4Cache), ctypes.POINTER(Tail), _I, _P, _I64P, _P, _I64P,
+                                       _P]),
+    "fq_dequant_int8": (ctypes.c_int, [ctypes.POINTER(Int4Cache), ctypes.POINTER(Tail), _I, _P, _I64P, _P, _I64P,
+                                       _P]),
     "fq_turbo_cache_append": (ctypes.c_int, [ctypes.POINTER(TurboCache), _P, _I64P, _P, _I64P, _I, _P, _I64P, _P,
                                              _I64P, _I, _P, _I64P, _P, _I64P, _I, _I, _P]),
     "fq_quest_decode_turbo": (ctypes.c_int, [ctypes.POINTER(TurboCache), _P, _I64P, _P, _I64P, ctypes.POINTER(Query),

@@ -16,6 +16,7 @@ import torch
 from transformers.cache_utils import Cache
 
 from .. import _lib as L
+from ..kernel.rotary import rotate, rotate_append
 
 
 class PagedKVCache(Cache):
@@ -81,12 +82,8 @@ class PagedKVCache(Cache):
                 "K_partial": self.K_partial[layer_idx, :, :, :tail, :],
                 "V_partial": self.V_partial[layer_idx, :, :, :tail, :]}
 
-    def update_quantized(self, K_new: torch.Tensor, V_new: torch.Tensor, layer_idx: int) -> None:
-        """Append K_new, V_new (B, H_kv, S_new, D) to layer ``layer_idx``: the
-        pages they complete are quantised into the cache, the remaining tokens
-        wait in the layer's bf16 tail."""
-        self._check_layer(layer_idx)
-        seen = self._seen_tokens[layer_idx]
+    def _check_new(self, K_new, V_new, seen) -> int:
+        """The tokens of an append to a layer that holds ``seen``; raises where they do not fit."""
         if K_new.shape != V_new.shape or K_new.dim() != 4:
             raise ValueError(f"{self._name}: K_new / V_new must share one (B, H_kv, S_new, D) shape; "
                              f"got {tuple(K_new.shape)} and {tuple(V_new.shape)}")
@@ -97,6 +94,15 @@ class PagedKVCache(Cache):
         if seen + S_new > self.max_seq_len:
             raise RuntimeError(f"{self._name}: {seen} cached + {S_new} new tokens exceeds max_seq_len="
                                f"{self.max_seq_len}")
+        return S_new
+
+    def update_quantized(self, K_new: torch.Tensor, V_new: torch.Tensor, layer_idx: int) -> None:
+        """Append K_new, V_new (B, H_kv, S_new, D) to layer ``layer_idx``: the
+        pages they complete are quantised into the cache, the remaining tokens
+        wait in the layer's bf16 tail."""
+        self._check_layer(layer_idx)
+        seen = self._seen_tokens[layer_idx]
+        S_new = self._check_new(K_new, V_new, seen)
         if S_new == 0:
             return
         if self._kernel_append and K_new.dtype == V_new.dtype == self.K_partial.dtype:
@@ -105,6 +111,30 @@ class PagedKVCache(Cache):
         else:
             self._append_stream(layer_idx, seen, K_new, V_new)
         self._seen_tokens[layer_idx] = seen + S_new
+
+    def buffers(self, layer_idx: int) -> dict:
+        """Layer ``layer_idx``'s planes and partial page at their full capacity, as rotate_append takes them."""
+        self._check_layer(layer_idx)
+        return {name: getattr(self, name)[layer_idx] for name in self._planes + ("K_partial", "V_partial")}
+
+    _planes: tuple = ()
+
+    def update_rotated(self, Q_new: torch.Tensor, K_new: torch.Tensor, V_new: torch.Tensor, cos: torch.Tensor,
+                       sin: torch.Tensor, layer_idx: int) -> torch.Tensor:
+        """update_quantized with the rotary embedding applied on the way: K_new rotated by cos / sin (B or 1,
+        S_new, R) of the tokens' positions and appended with V_new, and Q_new (B, H_q, S_new, D) rotated and
+        returned.  One launch on the INT4 and INT8 caches' kernel layout with tokens in the tail's type; otherwise
+        the rotation, then update_quantized."""
+        self._check_layer(layer_idx)
+        seen = self._seen_tokens[layer_idx]
+        self._check_new(K_new, V_new, seen)
+        if self._kernel_append and Q_new.dtype == K_new.dtype == V_new.dtype == self.K_partial.dtype:
+            out = rotate_append(Q_new, K_new, V_new, cos, sin, self.buffers(layer_idx), seen, page_size=self.page_size)
+            self._seen_tokens[layer_idx] = seen + K_new.shape[2]
+            return out
+        out, k = rotate(Q_new, K_new, cos, sin)
+        self.update_quantized(k, V_new, layer_idx)
+        return out
 
     def _append_stream(self, layer_idx, seen, K_new, V_new):
         """Other geometries, or new tokens in another dtype than the tail: the

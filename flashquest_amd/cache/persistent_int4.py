@@ -25,6 +25,7 @@ from ._paged import PagedKVCache
 class PersistentInt4KVCache(PagedKVCache):
     kv_bits = 4
     _name = "PersistentInt4KVCache"
+    _planes = ("K_packed", "K_scale", "K_mn", "V_packed", "V_scale", "V_mn")
 
     def __init__(self, *, batch_size: int, num_layers: int, num_kv_heads: int, head_dim: int, max_seq_len: int,
                  page_size: int = 64, device: str | torch.device = "cuda", meta_dtype: torch.dtype = torch.bfloat16,

@@ -21,6 +21,7 @@ from ._paged import PagedKVCache
 class PersistentInt8KVCache(PagedKVCache):
     kv_bits = 8
     _name = "PersistentInt8KVCache"
+    _planes = ("K_uint8", "K_scale", "K_mn", "V_uint8", "V_scale", "V_mn")
     _zero_tail_after_append = True
 
     def __init__(self, *, batch_size: int, num_layers: int, num_kv_heads: int, head_dim: int, max_seq_len: int,

@@ -20,6 +20,8 @@ from ._paged import PagedKVCache
 class PersistentTurboKVCache(PagedKVCache):
     kv_bits = 3
     _name = "PersistentTurboKVCache"
+    _planes = ("K_msb", "K_lsb", "K_scale_turbo", "V_msb", "V_lsb", "V_scale_turbo", "K_scale_raw",
+               "K_mn_raw")
 
     def __init__(self, *, batch_size: int, num_layers: int, num_kv_heads: int, head_dim: int, max_seq_len: int,
                  page_size: int = 64, device: str | torch.device = "cuda"):

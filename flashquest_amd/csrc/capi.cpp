@@ -939,6 +939,123 @@ int fq_int8_cache_append(const fq_int8_cache* cache, int32_t layer, void* k_part
                            kn_strides, v_new, vn_strides, seen, S_new, stream);
 }
 
+// A rotary descriptor for B x S tokens of D channels in `dtype`: angles and queries.
+static int check_rotary(const fq_rotary* r, int dtype, int B, int S, int D) {
+    if (!r) return fail(FQ_ERR_INVALID, "rotary descriptor is NULL");
+    if (r->R < 2 || r->R > D || r->R % 16)
+        return fail(FQ_ERR_UNSUPPORTED, "%d rotated channels of %d (a multiple of 16)", r->R, D);
+    if (r->H_q < 0) return fail(FQ_ERR_INVALID, "H_q=%d", r->H_q);
+    if (B == 0 || S == 0) return FQ_OK;
+    if (r->dtype != FQ_F32 && r->dtype != dtype)
+        return fail(FQ_ERR_UNSUPPORTED, "cos / sin must be fp32 or of the tokens' type");
+    if (!r->cos || !r->sin || (r->H_q && (!r->q || !r->q_out))) return fail(FQ_ERR_INVALID, "NULL tensor");
+    const int es = r->dtype == FQ_F32 ? 4 : 2;
+    if (r->cos_strides[2] != 1 || r->sin_strides[2] != 1 || !rows_aligned16(r->cos, r->cos_strides, 2, es) ||
+        !rows_aligned16(r->sin, r->sin_strides, 2, es))
+        return fail(FQ_ERR_UNSUPPORTED, "cos / sin need 16-byte aligned contiguous rows");
+    if (r->H_q && (r->q_strides[3] != 1 || r->qo_strides[3] != 1 || !rows_aligned16(r->q, r->q_strides, 3, 2) ||
+                   !rows_aligned16(r->q_out, r->qo_strides, 3, 2)))
+        return fail(FQ_ERR_UNSUPPORTED, "queries need 16-byte aligned contiguous rows");
+    return FQ_OK;
+}
+
+static int kv_cache_append_rotated(const fq_int4_cache* cache, int bits, int32_t layer, void* k_partial,
+                                   const int64_t kpart_strides[5], void* v_partial, const int64_t vpart_strides[5],
+                                   int32_t partial_dtype, const void* k_new, const int64_t kn_strides[4],
+                                   const void* v_new, const int64_t vn_strides[4], int32_t seen, int32_t S_new,
+                                   const fq_rotary* rotary, fq_stream_t stream) {
+    Int4Cache c{};
+    int st = check_cache(cache, &c, bits);
+    if (st) return st;
+    st = check_append(c.L, c.S, c.P, c.page, layer, k_partial, kpart_strides, v_partial, vpart_strides, partial_dtype,
+                      k_new, kn_strides, v_new, vn_strides, seen, S_new);
+    if (st) return st;
+    if (((uintptr_t)c.vsc | (uintptr_t)c.vmn) & 1) return fail(FQ_ERR_UNSUPPORTED, "V metadata must be 2-byte aligned");
+    st = check_rotary(rotary, partial_dtype, c.B, S_new, c.D);
+    if (st || S_new == 0) return st;
+    return hip_status(launch_rotate_append(c, layer, k_partial, kpart_strides, v_partial, vpart_strides, partial_dtype,
+                                           k_new, kn_strides, v_new, vn_strides, seen, S_new, *rotary,
+                                           (hipStream_t)stream),
+                      "cache append with rotation");
+}
+
+int fq_int4_cache_append_rotated(const fq_int4_cache* cache, int32_t layer, void* k_partial,
+                                 const int64_t kpart_strides[5], void* v_partial, const int64_t vpart_strides[5],
+                                 int32_t partial_dtype, const void* k_new, const int64_t kn_strides[4],
+                                 const void* v_new, const int64_t vn_strides[4], int32_t seen, int32_t S_new,
+                                 const fq_rotary* rotary, fq_stream_t stream) {
+    return kv_cache_append_rotated(cache, 4, layer, k_partial, kpart_strides, v_partial, vpart_strides, partial_dtype,
+                                   k_new, kn_strides, v_new, vn_strides, seen, S_new, rotary, stream);
+}
+
+int fq_int8_cache_append_rotated(const fq_int8_cache* cache, int32_t layer, void* k_partial,
+                                 const int64_t kpart_strides[5], void* v_partial, const int64_t vpart_strides[5],
+                                 int32_t partial_dtype, const void* k_new, const int64_t kn_strides[4],
+                                 const void* v_new, const int64_t vn_strides[4], int32_t seen, int32_t S_new,
+                                 const fq_rotary* rotary, fq_stream_t stream) {
+    return kv_cache_append_rotated(cache, 8, layer, k_partial, kpart_strides, v_partial, vpart_strides, partial_dtype,
+                                   k_new, kn_strides, v_new, vn_strides, seen, S_new, rotary, stream);
+}
+
+int fq_rotate(const fq_rotary* rotary, const void* k, const int64_t k_strides[4], void* k_out,
+              const int64_t ko_strides[4], int32_t dtype, int32_t B, int32_t H_kv, int32_t S, int32_t D,
+              fq_stream_t stream) {
+    if (D != 64 && D != 128) return fail(FQ_ERR_UNSUPPORTED, "head_dim=%d not in (64, 128)", D);
+    if (dtype != FQ_BF16 && dtype != FQ_F16) return fail(FQ_ERR_UNSUPPORTED, "tokens must be bf16 or fp16");
+    if (B < 0 || H_kv < 0 || S < 0) return fail(FQ_ERR_INVALID, "negative size");
+    const int st = check_rotary(rotary, dtype, B, S, D);
+    if (st || B == 0 || S == 0) return st;
+    if (H_kv) {
+        if (!k || !k_out) return fail(FQ_ERR_INVALID, "NULL tensor");
+        if (k_strides[3] != 1 || ko_strides[3] != 1 || !rows_aligned16(k, k_strides, 3, 2) ||
+            !rows_aligned16(k_out, ko_strides, 3, 2))
+            return fail(FQ_ERR_UNSUPPORTED, "keys need 16-byte aligned contiguous rows");
+    }
+    return hip_status(launch_rotate(*rotary, k, k_strides, k_out, ko_strides, dtype, B, H_kv, S, D, (hipStream_t)stream),
+                      "rotation");
+}
+
+static int dequant_cache(const fq_int4_cache* cache, const fq_tail* tail, int32_t start, void* k,
+                         const int64_t k_strides[4], void* v, const int64_t v_strides[4], fq_stream_t stream,
+                         int bits) {
+    Int4Cache c{};
+    const int st = check_cache(cache, &c, bits, true);
+    if (st) return st;
+    if (c.L != 1) return fail(FQ_ERR_INVALID, "one layer's cache view is read (L=%d)", c.L);
+    if (c.S > 0 && c.page != 64) return fail(FQ_ERR_UNSUPPORTED, "page_size=%d (64 only)", c.page);
+    if (c.S % 64) return fail(FQ_ERR_INVALID, "S=%d is not whole 64-token pages", c.S);
+    if ((int64_t)c.P * 64 < c.S) return fail(FQ_ERR_INVALID, "%d pages of 64 tokens < S=%d", c.P, c.S);
+    if (((uintptr_t)c.vsc | (uintptr_t)c.vmn) & 1) return fail(FQ_ERR_UNSUPPORTED, "V metadata must be 2-byte aligned");
+    TailArgs t{};
+    if (tail && tail->len > 0) {
+        if (tail->len >= 64) return fail(FQ_ERR_INVALID, "%d rows in the partial page", tail->len);
+        if (tail->D != c.D || !tail->k || !tail->v) return fail(FQ_ERR_INVALID, "tail of %d channels, cache of %d", tail->D, c.D);
+        if (tail->dtype != FQ_BF16) return fail(FQ_ERR_UNSUPPORTED, "the tail must be bf16");
+        if (tail->k_strides[4] != 1 || tail->v_strides[4] != 1 || !rows_aligned16(tail->k, tail->k_strides, 4, 2) ||
+            !rows_aligned16(tail->v, tail->v_strides, 4, 2))
+            return fail(FQ_ERR_UNSUPPORTED, "tails need 16-byte aligned contiguous rows");
+        t.k = tail->k; t.v = tail->v; t.dtype = tail->dtype; t.len = tail->len;
+        for (int i = 0; i < 4; ++i) { t.ks[i] = tail->k_strides[i]; t.vs[i] = tail->v_strides[i]; }
+    }
+    if (start < 0 || start > c.S + t.len) return fail(FQ_ERR_INVALID, "start=%d outside the %d tokens", start, c.S + t.len);
+    if (start == c.S + t.len) return FQ_OK;
+    if (!k || !v) return fail(FQ_ERR_INVALID, "NULL output");
+    if (k_strides[3] != 1 || v_strides[3] != 1 || !rows_aligned16(k, k_strides, 3, 2) || !rows_aligned16(v, v_strides, 3, 2))
+        return fail(FQ_ERR_UNSUPPORTED, "outputs need 16-byte aligned contiguous rows");
+    if ((int64_t)c.B * c.Hkv > 65535) return fail(FQ_ERR_UNSUPPORTED, "batch x KV heads > 65535");
+    return hip_status(launch_dequant_cache(c, t, start, k, k_strides, v, v_strides, (hipStream_t)stream), "cache read");
+}
+
+int fq_dequant_int4(const fq_int4_cache* cache, const fq_tail* tail, int32_t start, void* k,
+                    const int64_t k_strides[4], void* v, const int64_t v_strides[4], fq_stream_t stream) {
+    return dequant_cache(cache, tail, start, k, k_strides, v, v_strides, stream, 4);
+}
+
+int fq_dequant_int8(const fq_int8_cache* cache, const fq_tail* tail, int32_t start, void* k,
+                    const int64_t k_strides[4], void* v, const int64_t v_strides[4], fq_stream_t stream) {
+    return dequant_cache(cache, tail, start, k, k_strides, v, v_strides, stream, 8);
+}
+
 int fq_turbo_cache_append(const fq_turbo_cache* cache, void* k_scale_raw, const int64_t ksr_strides[5],
                           void* k_mn_raw, const int64_t kmr_strides[5], int32_t layer, void* k_partial,
                           const int64_t kpart_strides[5], void* v_partial, const int64_t vpart_strides[5],

@@ -310,6 +310,15 @@ hipError_t launch_turbo_append(const fq_turbo_cache& tc, const Int4Cache& raw, i
                                const int64_t* kpart_s, void* vpart, const int64_t* vpart_s, int part_dtype,
                                const void* knew, const int64_t* kn_s, const void* vnew, const int64_t* vn_s, int seen,
                                int S_new, hipStream_t st);
+// Appends with rotated keys and queries, the rotation alone, the cache as values (rotary.hip).
+hipError_t launch_rotate_append(const Int4Cache& c, int layer, void* kpart, const int64_t* kpart_s, void* vpart,
+                                const int64_t* vpart_s, int dtype, const void* knew, const int64_t* kn_s,
+                                const void* vnew, const int64_t* vn_s, int seen, int S_new, const fq_rotary& f,
+                                hipStream_t st);
+hipError_t launch_rotate(const fq_rotary& f, const void* k, const int64_t* k_s, void* k_out, const int64_t* ko_s,
+                         int dtype, int B, int H_kv, int S, int D, hipStream_t st);
+hipError_t launch_dequant_cache(const Int4Cache& c, const TailArgs& t, int start, void* k, const int64_t* k_s,
+                                void* v, const int64_t* v_s, hipStream_t st);
 // Fused-layout TurboQuant attention (turbo_fused.hip): D = 128, 64-token pages,
 // <= 3 query heads per KV head.  raw + sel: score and select in the kernel.
 bool turbo_fused_supported(const fq_turbo_cache& c, const QueryArgs& q);

@@ -4,6 +4,7 @@ from .kv_quant import (  # noqa: F401
     quantize_k_turbo, quantize_v, quantize_v_int4, quantize_v_turbo,
 )
 from .prefill import flash_attn_prefill_int4, flash_attn_prefill_int8, flash_attn_prefill_turbo  # noqa: F401
+from .rotary import dequantize_cache, rotate, rotate_append  # noqa: F401
 from .sparse_fwd import flash_attn_sparse_fwd  # noqa: F401
 from .sparse_int4_fwd import flash_attn_sparse_int4_fwd  # noqa: F401
 from .sparse_int4_fwd_compact import flash_attn_sparse_int4_fwd_compact  # noqa: F401

@@ -272,6 +272,56 @@ int fq_turbo_cache_append(const fq_turbo_cache* cache, void* k_scale_raw, const 
                           const void* v_new, const int64_t vn_strides[4],
                           int32_t seen, int32_t S_new, fq_stream_t stream);
 
+/* Rotary position embedding of a step's tokens (no single reference operator: transformers'
+ * apply_rotary_pos_emb, called before update_quantized by llama_persistent_patch.py:186-194):
+ * cos / sin (B, S_new, R), a batch stride of 0 for positions that the batch shares, channels
+ * contiguous, rows 16-byte aligned, R a multiple of 16 up to D; a row x becomes
+ *   y[i] = x[i] cos[i] - x[i + R/2] sin[i],  y[i + R/2] = x[i + R/2] cos[i + R/2] + x[i] sin[i + R/2]
+ * for i < R/2, channels R .. D - 1 unchanged, in fp32 (every product and sum rounded once)
+ * and rounded to the tokens' type.  q (B, H_q, S_new, D) -> q_out, the tokens' type, 16-byte
+ * aligned contiguous rows. */
+typedef struct fq_rotary {
+    const void* cos; int64_t cos_strides[3];
+    const void* sin; int64_t sin_strides[3];
+    int32_t dtype;          /* of cos and sin: FQ_F32 or the tokens' type */
+    int32_t R;
+    const void* q;   int64_t q_strides[4];
+    void* q_out;     int64_t qo_strides[4];
+    int32_t H_q;
+} fq_rotary;
+
+/* fq_int4_cache_append / fq_int8_cache_append of rotated keys, and the rotated queries, in one
+ * launch: bit-identical to rotating q and K_new first.  The partial tail, q, K_new and V_new
+ * share one 16-bit type.  q_out must not overlap any input. */
+int fq_int4_cache_append_rotated(const fq_int4_cache* cache, int32_t layer,
+                                 void* k_partial, const int64_t kpart_strides[5],
+                                 void* v_partial, const int64_t vpart_strides[5], int32_t partial_dtype,
+                                 const void* k_new, const int64_t kn_strides[4],
+                                 const void* v_new, const int64_t vn_strides[4],
+                                 int32_t seen, int32_t S_new, const fq_rotary* rotary, fq_stream_t stream);
+int fq_int8_cache_append_rotated(const fq_int8_cache* cache, int32_t layer,
+                                 void* k_partial, const int64_t kpart_strides[5],
+                                 void* v_partial, const int64_t vpart_strides[5], int32_t partial_dtype,
+                                 const void* k_new, const int64_t kn_strides[4],
+                                 const void* v_new, const int64_t vn_strides[4],
+                                 int32_t seen, int32_t S_new, const fq_rotary* rotary, fq_stream_t stream);
+
+/* The rotation alone: the queries of `rotary` and K (B, H_kv, S, D) -> K_out, one 16-bit type
+ * (the append to a TurboQuant cache rotates first).  D is 64 or 128. */
+int fq_rotate(const fq_rotary* rotary, const void* k, const int64_t k_strides[4],
+              void* k_out, const int64_t ko_strides[4], int32_t dtype,
+              int32_t B, int32_t H_kv, int32_t S, int32_t D, fq_stream_t stream);
+
+/* Tokens [start, S + tail->len) of one layer's cache (L == 1, S completed tokens, whole 64-token
+ * pages; S may be 0) as bf16 K and V (B, H_kv, S + tail->len - start, D): dequantize_k_int4 /
+ * dequantize_v_int4 (kernel/kv_quant.py:174-215), dequantize_k / dequantize_v (64-97), then the
+ * bf16 tail rows (tail NULL: none), as llama_persistent_patch.py:143-156 puts them together.
+ * Outputs have contiguous 16-byte aligned rows. */
+int fq_dequant_int4(const fq_int4_cache* cache, const fq_tail* tail, int32_t start,
+                    void* k, const int64_t k_strides[4], void* v, const int64_t v_strides[4], fq_stream_t stream);
+int fq_dequant_int8(const fq_int8_cache* cache, const fq_tail* tail, int32_t start,
+                    void* k, const int64_t k_strides[4], void* v, const int64_t v_strides[4], fq_stream_t stream);
+
 /* The whole decode branch of the reference's attention patch for a step with
  * a partial page (llama_persistent_patch.py:202-240): score, select and
  * attend the completed pages, attend the tail densely
