@@ -74,6 +74,17 @@ class Rotary(ctypes.Structure):
     ]
 
 
+class SharedQuery(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("q_strides", _I64x4),
+        ("out", ctypes.c_void_p), ("o_strides", _I64x4),
+        ("lse", ctypes.c_void_p), ("lse_strides", _I64x3),
+        ("start", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+        ("B", ctypes.c_int32), ("H_q", ctypes.c_int32), ("S_q", ctypes.c_int32),
+        ("sm_scale", ctypes.c_float),
+    ]
+
+
 class Prefill(ctypes.Structure):
     _fields_ = [
         ("q", ctypes.c_void_p), ("q_strides", _I64x4),
@@ -196,6 +207,16 @@ SIGNATURES = {
     "fq_prefill_plan": (ctypes.c_int, [_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_I), ctypes.POINTER(_I)]),
     "fq_prefill_turbo": (ctypes.c_int, [ctypes.POINTER(TurboCache), ctypes.POINTER(Tail), ctypes.POINTER(Prefill),
                                         _P, ctypes.c_size_t, _P]),
+    # a prefix that a batch shares, and each sequence's own tokens
+    "fq_shared_prefix_int4": (ctypes.c_int, [ctypes.POINTER(Int4Cache), ctypes.POINTER(Tail),
+                                             ctypes.POINTER(Int4Cache), ctypes.POINTER(Tail),
+                                             ctypes.POINTER(SharedQuery), _P, ctypes.c_size_t, _P]),
+    "fq_shared_prefix_int8": (ctypes.c_int, [ctypes.POINTER(Int4Cache), ctypes.POINTER(Tail),
+                                             ctypes.POINTER(Int4Cache), ctypes.POINTER(Tail),
+                                             ctypes.POINTER(SharedQuery), _P, ctypes.c_size_t, _P]),
+    "fq_shared_prefix_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Int4Cache), ctypes.POINTER(Tail),
+                                                           ctypes.POINTER(Int4Cache), ctypes.POINTER(Tail),
+                                                           ctypes.POINTER(SharedQuery), _I]),
     "fq_prefill_turbo_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(TurboCache), ctypes.POINTER(Tail),
                                                            ctypes.POINTER(Prefill)]),
 }

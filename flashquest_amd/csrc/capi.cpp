@@ -1452,6 +1452,113 @@ int fq_prefill_int8(const fq_int8_cache* cache, const fq_tail* tail, const fq_pr
     return prefill(cache, tail, query, workspace, workspace_bytes, stream, 8);
 }
 
+// One side of the shared-prefix attention: a layer of whole pages and the bf16 partial page.
+static int check_shared_part(const fq_int4_cache* cache, const fq_tail* tail, int bits, const char* name, Int4Cache& c,
+                             TailArgs& t) {
+    const int st = check_cache(cache, &c, bits, true);
+    if (st) return st;
+    if (c.L != 1) return fail(FQ_ERR_INVALID, "%s: one layer's cache view is attended (L=%d)", name, c.L);
+    if (c.S > 0) {
+        if (c.page != 64) return fail(FQ_ERR_UNSUPPORTED, "%s: page_size=%d (64 only)", name, c.page);
+        if (c.S % 64) return fail(FQ_ERR_INVALID, "%s: S=%d is not whole 64-token pages", name, c.S);
+        if ((int64_t)c.P * 64 < c.S) return fail(FQ_ERR_INVALID, "%s: %d pages of 64 tokens < S=%d", name, c.P, c.S);
+        const int kal = c.D * bits / 32 >= 16 ? 16 : 8;
+        for (int i = 0; i < 4; ++i)
+            if (c.kp_s[i] % kal) return fail(FQ_ERR_UNSUPPORTED, "%s: K code strides must be multiples of %d bytes", name, kal);
+        if (!aligned(c.kp, kal)) return fail(FQ_ERR_UNSUPPORTED, "%s: K codes must be %d-byte aligned", name, kal);
+        if (!aligned(c.vsc, 2) || !aligned(c.vmn, 2))
+            return fail(FQ_ERR_UNSUPPORTED, "%s: V metadata must be 2-byte aligned", name);
+    }
+    t = TailArgs{};
+    if (tail && tail->len != 0) {
+        if (tail->len < 0 || tail->len >= 64) return fail(FQ_ERR_INVALID, "%s: %d rows in the partial page", name, tail->len);
+        if (!tail->k || !tail->v) return fail(FQ_ERR_INVALID, "%s: NULL tail", name);
+        if (tail->D != c.D) return fail(FQ_ERR_INVALID, "%s: tail of %d channels, cache of %d", name, tail->D, c.D);
+        if (tail->dtype != FQ_BF16) return fail(FQ_ERR_UNSUPPORTED, "%s: the tail must be bf16", name);
+        if (tail->k_strides[4] != 1 || tail->v_strides[4] != 1 || !rows_aligned16(tail->k, tail->k_strides, 4, 2) ||
+            !rows_aligned16(tail->v, tail->v_strides, 4, 2))
+            return fail(FQ_ERR_UNSUPPORTED, "%s: tails need 16-byte aligned contiguous rows", name);
+        t.k = tail->k; t.v = tail->v; t.dtype = tail->dtype; t.len = tail->len;
+        for (int i = 0; i < 4; ++i) { t.ks[i] = tail->k_strides[i]; t.vs[i] = tail->v_strides[i]; }
+    }
+    return FQ_OK;
+}
+
+// pointers false: the sizes only (q, out and the workspace may not be there yet)
+static int check_shared(const fq_int4_cache* prefix, const fq_tail* prefix_tail, const fq_int4_cache* suffix,
+                        const fq_tail* suffix_tail, const fq_shared_query* q, int bits, bool pointers, Int4Cache& pc,
+                        TailArgs& pt, Int4Cache& sc, TailArgs& st_) {
+    int st = check_shared_part(prefix, prefix_tail, bits, "prefix", pc, pt);
+    if (st) return st;
+    st = check_shared_part(suffix, suffix_tail, bits, "suffix", sc, st_);
+    if (st) return st;
+    if (!q) return fail(FQ_ERR_INVALID, "query descriptor is NULL");
+    if (pc.B != 1) return fail(FQ_ERR_INVALID, "the prefix is one sequence (B=%d)", pc.B);
+    if (q->B < 1 || sc.B != q->B) return fail(FQ_ERR_INVALID, "%d sequences of queries, %d of own tokens", q->B, sc.B);
+    if (pc.Hkv != sc.Hkv || pc.D != sc.D)
+        return fail(FQ_ERR_INVALID, "prefix (%d heads x %d) and suffix (%d x %d) differ", pc.Hkv, pc.D, sc.Hkv, sc.D);
+    if (pc.S > 0 && sc.S > 0 && pc.meta_dtype != sc.meta_dtype)
+        return fail(FQ_ERR_UNSUPPORTED, "prefix and suffix metadata must have one type");
+    if (q->H_q < 1 || q->H_q % pc.Hkv) return fail(FQ_ERR_INVALID, "H_q=%d must be divisible by H_kv=%d", q->H_q, pc.Hkv);
+    if (pc.S + pt.len < 1) return fail(FQ_ERR_INVALID, "the prefix has no tokens");
+    if (q->S_q < 1 || sc.S + st_.len < q->S_q)
+        return fail(FQ_ERR_INVALID, "S_q=%d query tokens, the suffix has %d (they are its last)", q->S_q, sc.S + st_.len);
+    if ((int64_t)q->B * q->H_q * q->S_q > 0x7FFFFFFF / 64) return fail(FQ_ERR_UNSUPPORTED, "too many query rows");
+    if (!is_half(q->dtype)) return fail(FQ_ERR_UNSUPPORTED, "queries must be bf16 or fp16");
+    if (pc.S == 0) pc.meta_dtype = sc.meta_dtype;
+    if (!pointers) return FQ_OK;
+    if (!q->q || !q->out) return fail(FQ_ERR_INVALID, "query/output is NULL");
+    if (q->q_strides[3] != 1 || !rows_aligned16(q->q, q->q_strides, 3, 2))
+        return fail(FQ_ERR_UNSUPPORTED, "queries need 16-byte aligned contiguous rows");
+    if (q->o_strides[3] != 1 || !aligned(q->out, 8)) return fail(FQ_ERR_UNSUPPORTED, "outputs need 8-byte aligned contiguous rows");
+    for (int i = 0; i < 3; ++i)
+        if (q->o_strides[i] % 4) return fail(FQ_ERR_UNSUPPORTED, "output strides must be multiples of 4 elements");
+    if (!aligned(q->start, 4)) return fail(FQ_ERR_INVALID, "start must be int32");
+    return FQ_OK;
+}
+
+static int shared_prefix(const fq_int4_cache* prefix, const fq_tail* prefix_tail, const fq_int4_cache* suffix,
+                         const fq_tail* suffix_tail, const fq_shared_query* q, void* workspace,
+                         size_t workspace_bytes_, fq_stream_t stream, int bits) {
+    Int4Cache pc{}, sc{};
+    TailArgs pt{}, st_{};
+    const int st = check_shared(prefix, prefix_tail, suffix, suffix_tail, q, bits, true, pc, pt, sc, st_);
+    if (st) return st;
+    size_t need = 0;
+    hipError_t e = launch_shared_prefix(pc, pt, sc, st_, *q, 0.f, nullptr, &need, nullptr);
+    if (e != hipSuccess) return hip_status(e, "shared prefix plan");
+    if (!workspace || workspace_bytes_ < need)
+        return fail(FQ_ERR_WORKSPACE, "shared prefix workspace of %zu bytes needed (got %zu)", need, workspace_bytes_);
+    if (!aligned(workspace, 16)) return fail(FQ_ERR_INVALID, "workspace must be 16-byte aligned");
+    const float sm = q->sm_scale > 0.f ? q->sm_scale : 1.0f / sqrtf((float)pc.D);
+    return hip_status(launch_shared_prefix(pc, pt, sc, st_, *q, sm * kLog2e, workspace, &need, (hipStream_t)stream),
+                      "shared prefix attention");
+}
+
+int fq_shared_prefix_int4(const fq_int4_cache* prefix, const fq_tail* prefix_tail, const fq_int4_cache* suffix,
+                          const fq_tail* suffix_tail, const fq_shared_query* query, void* workspace,
+                          size_t workspace_bytes, fq_stream_t stream) {
+    return shared_prefix(prefix, prefix_tail, suffix, suffix_tail, query, workspace, workspace_bytes, stream, 4);
+}
+
+int fq_shared_prefix_int8(const fq_int8_cache* prefix, const fq_tail* prefix_tail, const fq_int8_cache* suffix,
+                          const fq_tail* suffix_tail, const fq_shared_query* query, void* workspace,
+                          size_t workspace_bytes, fq_stream_t stream) {
+    return shared_prefix(prefix, prefix_tail, suffix, suffix_tail, query, workspace, workspace_bytes, stream, 8);
+}
+
+size_t fq_shared_prefix_workspace_bytes(const fq_int4_cache* prefix, const fq_tail* prefix_tail,
+                                        const fq_int4_cache* suffix, const fq_tail* suffix_tail,
+                                        const fq_shared_query* query, int32_t bits) {
+    Int4Cache pc{}, sc{};
+    TailArgs pt{}, st_{};
+    size_t need = 0;
+    if (bits != 4 && bits != 8) return 0;
+    if (check_shared(prefix, prefix_tail, suffix, suffix_tail, query, bits, false, pc, pt, sc, st_)) return 0;
+    if (launch_shared_prefix(pc, pt, sc, st_, *query, 0.f, nullptr, &need, nullptr) != hipSuccess) return 0;
+    return need;
+}
+
 int fq_quest_decode_int4_noalloc(const fq_int4_cache* cache, const fq_query* query, const float* retention,
                                  int32_t num_sinks, int32_t window_pages, int32_t k_max, int32_t select_mode,
                                  float* scores_out, uint8_t* mask_out, fq_stream_t stream) {

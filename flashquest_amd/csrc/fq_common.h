@@ -319,6 +319,10 @@ hipError_t launch_rotate(const fq_rotary& f, const void* k, const int64_t* k_s, 
                          int dtype, int B, int H_kv, int S, int D, hipStream_t st);
 hipError_t launch_dequant_cache(const Int4Cache& c, const TailArgs& t, int start, void* k, const int64_t* k_s,
                                 void* v, const int64_t* v_s, hipStream_t st);
+// Attention over a shared prefix and each sequence's own tokens (shared_prefix.hip); ws null: only
+// the workspace bytes.
+hipError_t launch_shared_prefix(const Int4Cache& pc, const TailArgs& pt, const Int4Cache& sc, const TailArgs& st_,
+                                const fq_shared_query& q, float qk_scale, void* ws, size_t* bytes, hipStream_t st);
 // Fused-layout TurboQuant attention (turbo_fused.hip): D = 128, 64-token pages,
 // <= 3 query heads per KV head.  raw + sel: score and select in the kernel.
 bool turbo_fused_supported(const fq_turbo_cache& c, const QueryArgs& q);

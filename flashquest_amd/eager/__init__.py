@@ -9,4 +9,5 @@ from .decode import (  # noqa: F401
 )
 from .page_summary import compute_page_summary  # noqa: F401
 from .prefill import prefill_attention_layer  # noqa: F401
+from .shared_prefix import shared_prefix_attention  # noqa: F401
 from .selection import build_compact_selection, select_pages, select_pages_vectorized  # noqa: F401

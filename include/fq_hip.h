@@ -607,6 +607,41 @@ int fq_prefill_int8(const fq_int8_cache* cache, const fq_tail* tail, const fq_pr
  * fq_prefill_turbo_workspace_bytes (dense bf16 K and V^T of the attended keys). */
 int fq_prefill_turbo(const fq_turbo_cache* cache, const fq_tail* tail, const fq_prefill* query,
                      void* workspace, size_t workspace_bytes, fq_stream_t stream);
+
+/* Queries and outputs of a step of B sequences that share a prefix: Q, O (B, H_q, S_q, D), one
+ * 16-bit type, lse (B, H_q, S_q) or NULL.  start: (B) int32 on the device, the first of a
+ * sequence's own tokens that is not padding (clamped to 0 .. the suffix's tokens), or NULL. */
+typedef struct fq_shared_query {
+    const void* q; int64_t q_strides[4];   /* rows contiguous, 16-byte aligned */
+    void* out;     int64_t o_strides[4];   /* rows contiguous, 8-byte aligned */
+    float* lse;    int64_t lse_strides[3];
+    const int32_t* start;
+    int32_t dtype;
+    int32_t B, H_q, S_q;
+    float sm_scale;                        /* <= 0 selects 1/sqrt(D) */
+} fq_shared_query;
+
+/* Attention over a prefix that B sequences share and each sequence's own tokens (no reference
+ * counterpart; a cache per sequence, as the reference holds them, would keep and read the
+ * prefix B times):
+ *   O[b, :, i] = softmax(q [K_prefix; K_suffix[b]]^T sm_scale) [V_prefix; V_suffix[b]]
+ * over all prefix tokens and the suffix tokens start[b] <= j <= S_suffix - S_q + i (the S_q query
+ * tokens are the suffix's last S_q).  prefix: one layer, B == 1; suffix: one layer, B sequences;
+ * each with S completed tokens (whole 64-token pages, may be 0) and the bf16 rows of its partial
+ * page (tail NULL or len 0: none).  At least one prefix token and S_q suffix tokens.  D is 64 or
+ * 128; the two caches have one metadata type.  K code rows are 16-byte aligned (INT4 with
+ * D == 64: 8).  K values up to 2e6 and V values up to 3e4 in size.  Two or three launches;
+ * every byte of the workspace is written before it is read.  Deterministic. */
+int fq_shared_prefix_int4(const fq_int4_cache* prefix, const fq_tail* prefix_tail,
+                          const fq_int4_cache* suffix, const fq_tail* suffix_tail, const fq_shared_query* query,
+                          void* workspace, size_t workspace_bytes, fq_stream_t stream);
+int fq_shared_prefix_int8(const fq_int8_cache* prefix, const fq_tail* prefix_tail,
+                          const fq_int8_cache* suffix, const fq_tail* suffix_tail, const fq_shared_query* query,
+                          void* workspace, size_t workspace_bytes, fq_stream_t stream);
+/* Bytes of workspace for those arguments (bits 4 or 8); 0 when they would be refused. */
+size_t fq_shared_prefix_workspace_bytes(const fq_int4_cache* prefix, const fq_tail* prefix_tail,
+                                        const fq_int4_cache* suffix, const fq_tail* suffix_tail,
+                                        const fq_shared_query* query, int32_t bits);
 /* No reference counterpart: workspace bytes of fq_prefill_turbo (0 for invalid arguments). */
 size_t fq_prefill_turbo_workspace_bytes(const fq_turbo_cache* cache, const fq_tail* tail, const fq_prefill* query);
 
