@@ -48,6 +48,13 @@ struct Entries {
     decltype(&fq_quantize_k_int8) quant_k8;
     decltype(&fq_quantize_v_int4) quant_v4;
     decltype(&fq_quantize_v_int8) quant_v8;
+    decltype(&fq_int4_cache_append_rotated) rotated4;
+    decltype(&fq_int8_cache_append_rotated) rotated8;
+    decltype(&fq_dequant_int4) dequant4;
+    decltype(&fq_dequant_int8) dequant8;
+    decltype(&fq_shared_prefix_int4) shared4;
+    decltype(&fq_shared_prefix_int8) shared8;
+    decltype(&fq_shared_prefix_workspace_bytes) ws_shared;
 };
 Entries g_fq{};
 
@@ -357,6 +364,197 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// One layer of an INT4 or INT8 cache, given by name: its planes and its partial page.
+struct Layer {
+    int bits = 0;
+    const at::Tensor* t[6] = {};         // K codes, K scale, K min, V codes, V scale, V min
+    const at::Tensor* kp = nullptr;
+    const at::Tensor* vp = nullptr;
+    fq_int4_cache c{};
+};
+
+// The tensors of a cache dict on `on` (any device: null), all 4D and of one (B, H_kv), metadata of `codes` tokens and
+// their pages.  page 64.
+bool layer_of(PyObject* dict, const at::Tensor* on, Layer& y) {
+    static const char* const names[2][6] = {{"K_packed", "K_scale", "K_mn", "V_packed", "V_scale", "V_mn"},
+                                            {"K_uint8", "K_scale", "K_mn", "V_uint8", "V_scale", "V_mn"}};
+    if (!PyDict_CheckExact(dict)) return false;
+    auto get = [&](const char* n) -> const at::Tensor* {
+        PyObject* o = PyDict_GetItemString(dict, n);
+        return o ? plain(o) : nullptr;
+    };
+    y.bits = PyDict_GetItemString(dict, "K_packed") ? 4 : 8;
+    for (int i = 0; i < 6; ++i)
+        if (!(y.t[i] = get(names[y.bits == 8][i])) || y.t[i]->dim() != 4) return false;
+    if (!(y.kp = get("K_partial")) || !(y.vp = get("V_partial")) || y.kp->dim() != 4) return false;
+    if (y.kp->sizes() != y.vp->sizes() || y.kp->scalar_type() != y.vp->scalar_type()) return false;
+    if (!int_cache(y.t, y.bits, 64, y.c)) return false;
+    const at::Device dev = on ? on->device() : y.kp->device();
+    const int64_t B = y.kp->size(0), H = y.kp->size(1), D = y.kp->size(3);
+    if (y.kp->device() != dev || y.vp->device() != dev || (D != 64 && D != 128) || y.c.D != D) return false;
+    for (int i = 0; i < 6; ++i)
+        if (y.t[i]->device() != dev || y.t[i]->size(0) != B || y.t[i]->size(1) != H) return false;
+    const int64_t S = y.t[0]->size(2), P = (S + 63) / 64;
+    return y.t[1]->size(2) >= P && y.t[2]->size(2) >= P && y.t[3]->size(2) == S && y.t[4]->size(2) == S &&
+           y.t[5]->size(2) == S && y.t[1]->size(3) == D && y.t[2]->size(3) == D && y.t[3]->size(3) == y.t[0]->size(3) &&
+           y.t[4]->size(3) == y.t[5]->size(3) && S <= 0x7FFFFFFF;
+}
+
+bool index_of(PyObject* o, int64_t& v) {         // a plain int that fits
+    if (!PyLong_CheckExact(o)) return false;
+    int over = 0;
+    v = PyLong_AsLongLongAndOverflow(o, &over);
+    return over == 0;
+}
+
+// rotate_append(q, k, v, cos, sin, cache, seen, current device, stream) -> rotated q, or None
+PyObject* rotate_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 9) return none();
+    const at::Tensor* x[5];
+    for (int i = 0; i < 5; ++i)
+        if (!(x[i] = plain(a[i])) || x[i]->device() != x[0]->device()) return none();
+    const at::Tensor &q = *x[0], &k = *x[1], &v = *x[2], &cs = *x[3], &sn = *x[4];
+    int64_t seen = 0, cur = -1;
+    if (!index_of(a[6], seen) || !index_of(a[7], cur) || cur != q.device().index()) return none();
+    if (q.dim() != 4 || k.dim() != 4 || k.sizes() != v.sizes() || cs.dim() != 3 || cs.sizes() != sn.sizes()) return none();
+    const int dt = dtype_code(q), ct = dtype_code(cs);
+    if ((dt != FQ_BF16 && dt != FQ_F16) || dtype_code(k) != dt || dtype_code(v) != dt || dtype_code(sn) != ct ||
+        (ct != FQ_F32 && ct != dt))
+        return none();
+    const int64_t B = q.size(0), Hq = q.size(1), S = q.size(2), D = q.size(3), Hkv = k.size(1), R = cs.size(2);
+    if (B < 1 || S < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || k.size(0) != B || k.size(2) != S || k.size(3) != D) return none();
+    if ((cs.size(0) != 1 && cs.size(0) != B) || cs.size(1) != S || R < 16 || R > D || R % 16) return none();
+    const int64_t ca = ct == FQ_F32 ? 4 : 8;
+    if (!rows(q, 8) || !rows(k, 8) || !rows(v, 8) || !rows(cs, ca) || !rows(sn, ca)) return none();
+    Layer y;
+    if (!layer_of(a[5], &q, y) || y.c.D != D || y.c.B != B || y.c.H_kv != Hkv || y.kp->size(2) != 64) return none();
+    if (dtype_code(*y.kp) != dt || seen < 0 || seen + S > y.c.S) return none();
+    at::Tensor out = at::empty(q.sizes(), q.options());
+    fq_rotary r{};
+    r.cos = cs.data_ptr(); strides(cs, r.cos_strides);
+    r.sin = sn.data_ptr(); strides(sn, r.sin_strides);
+    if (cs.size(0) == 1 && B > 1) r.cos_strides[0] = r.sin_strides[0] = 0;
+    r.dtype = ct;
+    r.R = (int)R;
+    r.q = q.data_ptr(); strides(q, r.q_strides);
+    r.q_out = out.data_ptr(); strides(out, r.qo_strides);
+    r.H_q = (int)Hq;
+    int64_t kps[5], vps[5], ks[4], vs[4];
+    strides(*y.kp, kps); strides(*y.vp, vps); strides(k, ks); strides(v, vs);
+    fq_stream_t st = (fq_stream_t)PyLong_AsVoidPtr(a[8]);
+    void *kp = y.kp->data_ptr(), *vp = y.vp->data_ptr();
+    const void *kn = k.data_ptr(), *vn = v.data_ptr();
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = (y.bits == 4 ? g_fq.rotated4 : g_fq.rotated8)(&y.c, 0, kp, kps, vp, vps, dt, kn, ks, vn, vs, (int)seen,
+                                                           (int)S, &r, st);
+    Py_END_ALLOW_THREADS
+    if (status != FQ_OK) return none();
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// The first `tokens` tokens of a layer: its descriptor's whole pages, and the partial page's rows.
+bool held_tokens(Layer& y, int64_t tokens, fq_tail& t) {
+    const int64_t rest = tokens % 64, done = tokens - rest;
+    if (done > y.c.S || done / 64 > y.t[1]->size(2) || done / 64 > y.t[2]->size(2) || rest > y.kp->size(2)) return false;
+    y.c.S = (int)done;
+    y.c.P = (int)(done / 64);
+    if (rest == 0) return true;
+    if (dtype_code(*y.kp) != FQ_BF16 || !rows(*y.kp, 8) || !rows(*y.vp, 8)) return false;
+    t.k = y.kp->data_ptr(); strides(*y.kp, t.k_strides);
+    t.v = y.vp->data_ptr(); strides(*y.vp, t.v_strides);
+    t.dtype = FQ_BF16;
+    t.len = (int)rest;
+    t.D = y.c.D;
+    return true;
+}
+
+// dequantize(cache, length, start, current device, stream) -> (K, V), or None
+PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t length = 0, start = 0, cur = -1;
+    Layer y;
+    if (n != 5 || !index_of(a[1], length) || !index_of(a[2], start) || !index_of(a[3], cur)) return none();
+    if (!layer_of(a[0], nullptr, y) || cur != y.kp->device().index()) return none();
+    fq_tail t{};
+    if (start < 0 || start >= length || length > 0x7FFFFFFF || !held_tokens(y, length, t)) return none();
+    const auto opt = y.kp->options().dtype(at::kBFloat16);
+    at::Tensor K = at::empty({y.c.B, y.c.H_kv, length - start, y.c.D}, opt), V = at::empty(K.sizes(), opt);
+    if (K.numel() == 0) return none();
+    int64_t s[4];
+    strides(K, s);
+    void *kd = K.data_ptr(), *vd = V.data_ptr();
+    fq_stream_t st = (fq_stream_t)PyLong_AsVoidPtr(a[4]);
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = (y.bits == 4 ? g_fq.dequant4 : g_fq.dequant8)(&y.c, &t, (int)start, kd, s, vd, s, st);
+    Py_END_ALLOW_THREADS
+    if (status != FQ_OK) return none();
+    return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(K)), THPVariable_Wrap(std::move(V)));
+    END_HANDLE_TH_ERRORS
+}
+
+// shared_prefix(q, prefix, suffix, start or None, sm_scale or None, return_lse, current device, stream)
+//   -> O or (O, lse), or None
+PyObject* shared_prefix(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 8) return none();
+    const at::Tensor* q = plain(a[0]);
+    int64_t cur = -1;
+    if (!q || q->dim() != 4 || !rows(*q, 8) || !index_of(a[6], cur) || cur != q->device().index()) return none();
+    const int dt = dtype_code(*q);
+    if ((dt != FQ_BF16 && dt != FQ_F16) || q->numel() == 0) return none();
+    const int64_t B = q->size(0), Hq = q->size(1), Sq = q->size(2), D = q->size(3);
+    Layer y[2];
+    fq_tail t[2] = {};
+    for (int i = 0; i < 2; ++i) {
+        if (!layer_of(a[1 + i], q, y[i]) || y[i].c.D != D || y[i].t[0]->size(2) % 64 || y[i].kp->size(2) >= 64) return none();
+        if (!held_tokens(y[i], y[i].t[0]->size(2) + y[i].kp->size(2), t[i])) return none();
+    }
+    const at::Tensor* start = nullptr;
+    if (a[3] != Py_None) {
+        start = plain(a[3]);
+        if (!start || start->device() != q->device() || start->dim() != 1 || start->size(0) != B || !rows(*start) ||
+            start->scalar_type() != at::kInt)
+            return none();
+    }
+    if (y[0].bits != y[1].bits || y[0].c.B != 1 || y[1].c.B != B || y[0].c.H_kv != y[1].c.H_kv) return none();
+    fq_shared_query p{};
+    if (a[4] != Py_None) {
+        p.sm_scale = (float)PyFloat_AsDouble(a[4]);
+        if (PyErr_Occurred()) PyErr_Clear();
+        if (!(p.sm_scale > 0.f)) return none();
+    }
+    const bool want_lse = a[5] == Py_True;
+    if (!want_lse && a[5] != Py_False) return none();
+    at::Tensor out = at::empty(q->sizes(), q->options()), lse;
+    p.q = q->data_ptr(); strides(*q, p.q_strides);
+    p.out = out.data_ptr(); strides(out, p.o_strides);
+    if (want_lse) {
+        lse = at::empty(q->sizes().slice(0, 3), q->options().dtype(at::kFloat));
+        p.lse = (float*)lse.data_ptr();
+        strides(lse, p.lse_strides);
+    }
+    p.start = start ? (const int32_t*)start->data_ptr() : nullptr;
+    p.dtype = dt;
+    p.B = (int)B; p.H_q = (int)Hq; p.S_q = (int)Sq;
+    const size_t bytes = g_fq.ws_shared(&y[0].c, &t[0], &y[1].c, &t[1], &p, y[0].bits);
+    if (bytes == 0) return none();
+    const at::Tensor ws = at::empty({(int64_t)bytes}, q->options().dtype(at::kByte));
+    void* w = ws.data_ptr();
+    fq_stream_t st = (fq_stream_t)PyLong_AsVoidPtr(a[7]);
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = (y[0].bits == 4 ? g_fq.shared4 : g_fq.shared8)(&y[0].c, &t[0], &y[1].c, &t[1], &p, w, bytes, st);
+    Py_END_ALLOW_THREADS
+    if (status != FQ_OK) return none();
+    if (!want_lse) return THPVariable_Wrap(std::move(out));
+    return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(lse)));
+    END_HANDLE_TH_ERRORS
+}
+
 // bind({entry name: address}): the library's entries; raises KeyError for a missing one.
 PyObject* bind(PyObject*, PyObject* table) {
     auto get = [&](const char* name) -> void* {
@@ -389,6 +587,13 @@ PyObject* bind(PyObject*, PyObject* table) {
     FQ_BIND(quant_k8, fq_quantize_k_int8)
     FQ_BIND(quant_v4, fq_quantize_v_int4)
     FQ_BIND(quant_v8, fq_quantize_v_int8)
+    FQ_BIND(rotated4, fq_int4_cache_append_rotated)
+    FQ_BIND(rotated8, fq_int8_cache_append_rotated)
+    FQ_BIND(dequant4, fq_dequant_int4)
+    FQ_BIND(dequant8, fq_dequant_int8)
+    FQ_BIND(shared4, fq_shared_prefix_int4)
+    FQ_BIND(shared8, fq_shared_prefix_int8)
+    FQ_BIND(ws_shared, fq_shared_prefix_workspace_bytes)
 #undef FQ_BIND
     g_fq = e;
     Py_RETURN_NONE;
@@ -399,6 +604,9 @@ PyMethodDef g_methods[] = {
     {"decode", (PyCFunction)(void (*)(void))decode, METH_FASTCALL, "One decode step, or None."},
     {"prefill", (PyCFunction)(void (*)(void))prefill, METH_FASTCALL, "One prefill, or None."},
     {"quantize", (PyCFunction)(void (*)(void))quantize, METH_FASTCALL, "One quantiser call, or None."},
+    {"rotate_append", (PyCFunction)(void (*)(void))rotate_append, METH_FASTCALL, "One rotated append, or None."},
+    {"dequantize", (PyCFunction)(void (*)(void))dequantize, METH_FASTCALL, "A cache layer as values, or None."},
+    {"shared_prefix", (PyCFunction)(void (*)(void))shared_prefix, METH_FASTCALL, "One shared-prefix step, or None."},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_fq_host", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -8,16 +8,17 @@ from __future__ import annotations
 
 import torch
 
+from .. import _host
 from .. import _lib as L
 from .. import _ops
-from ..kernel.rotary import _PLANES, cache_bits, on_device, same_device
+from ..kernel.rotary import _PLANES, _layer_planes, cache_bits, on_device, same_device
 
 
 def _check_part(name, views, bits, D):
     """(batch, KV heads, tokens) of a cache layer's views."""
-    planes = [views[n] for n in _PLANES[bits]]
+    planes = _layer_planes(views, bits)
     kt, vt = views["K_partial"], views["V_partial"]
-    if any(t.dim() != 4 for t in planes) or kt.dim() != 4 or kt.shape != vt.shape:
+    if kt.dim() != 4 or kt.shape != vt.shape:
         raise ValueError(f"{name}: one layer's views (B, H_kv, ...) are attended, K_partial and V_partial alike")
     B, H_kv, S, _ = planes[0].shape
     if kt.shape[:2] != (B, H_kv) or any(t.shape[:2] != (B, H_kv) for t in planes):
@@ -29,8 +30,6 @@ def _check_part(name, views, bits, D):
     width = D // 2 if bits == 4 else D
     if any(planes[i].shape[3] != w for i, w in ((0, width), (1, D), (2, D), (3, width))) or kt.shape[3] != D:
         raise ValueError(f"{name}: the cache does not hold head_dim {D}")
-    if planes[4].shape[3] != planes[5].shape[3]:
-        raise ValueError(f"{name}: V_scale and V_mn differ")
     if kt.shape[2] and (kt.dtype != torch.bfloat16 or vt.dtype != torch.bfloat16):
         raise NotImplementedError(f"{name}: the partial page must be bf16; got {kt.dtype}, {vt.dtype}")
     return B, H_kv, S + kt.shape[2]
@@ -66,6 +65,12 @@ def shared_prefix_attention(q: torch.Tensor, prefix: dict, suffix: dict, *, page
     Returns O (B, H_q, S_q, D) in q's type, with return_lse also the natural-log sum of exponentials (B, H_q, S_q)
     fp32.
     """
+    host = _host.module() if q.is_cuda and page_size == 64 else None
+    if host is not None:
+        res = host.shared_prefix(q, prefix, suffix, suffix_start, sm_scale, bool(return_lse),
+                                 torch.cuda.current_device(), L.stream_handle(q.device))
+        if res is not None:
+            return res
     if q.dim() != 4:
         raise ValueError(f"q must be (B, H_q, S_q, D); got {tuple(q.shape)}")
     B, H_q, S_q, D = q.shape

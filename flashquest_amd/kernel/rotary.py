@@ -17,6 +17,7 @@ import contextlib
 
 import torch
 
+from .. import _host
 from .. import _lib as L
 from .. import _ops
 
@@ -31,6 +32,22 @@ def cache_bits(cache: dict) -> int:
         if all(n in cache for n in names):
             return bits
     raise ValueError(f"not the buffers or views of an INT4, INT8 or TurboQuant cache layer: {sorted(cache)}")
+
+
+def _layer_planes(cache: dict, bits: int) -> list:
+    """The planes of one layer, their types checked (shapes are the callers')."""
+    planes = [cache[n] for n in _PLANES[bits]]
+    codes = (0, 3) if bits != 3 else (0, 1, 3, 4)
+    for i, (n, t) in enumerate(zip(_PLANES[bits], planes)):
+        if t.dim() != 4:
+            raise ValueError(f"{n} must be one layer's, (B, H_kv, ...); got {tuple(t.shape)}")
+        if (t.dtype == torch.uint8) != (i in codes) or (i not in codes and t.dtype not in (torch.bfloat16, torch.float16)):
+            raise AssertionError(f"{n}: codes are uint8, metadata bf16 or fp16; got {t.dtype}")
+        if bits == 3 and i not in codes and t.dtype != torch.bfloat16:
+            raise AssertionError(f"{n} must be bf16; got {t.dtype}")
+    if bits != 3 and planes[4].shape != planes[5].shape:
+        raise ValueError(f"V_scale and V_mn must share one shape; got {tuple(planes[4].shape)} and {tuple(planes[5].shape)}")
+    return planes
 
 
 def on_device(t: torch.Tensor):
@@ -122,10 +139,15 @@ def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.
 
     64-token pages and head_dim 64 or 128; other layouts raise NotImplementedError, before anything is changed.
     """
+    host = _host.module() if q.is_cuda and page_size == 64 else None
+    if host is not None:
+        out = host.rotate_append(q, k, v, cos, sin, cache, seen, torch.cuda.current_device(), L.stream_handle(q.device))
+        if out is not None:
+            return out
     _check_tokens(q, k, v, cos, sin)
     bits = cache_bits(cache)
     names = _PLANES[bits]
-    planes = [cache[n] for n in names]
+    planes = _layer_planes(cache, bits)
     kp, vp = cache["K_partial"], cache["V_partial"]
     B, H_q, S, D = q.shape
     H_kv = k.shape[1]
@@ -208,11 +230,16 @@ def dequantize_cache(cache: dict, length: int, *, start: int = 0, page_size: int
     dequantize_k / dequantize_v, 64-97), in one launch with the partial page's rows, as
     llama_persistent_patch.py:143-156 puts them together for its eager attention.
     """
+    host = _host.module() if page_size == 64 else None
+    if host is not None and cache.get("K_partial") is not None and cache["K_partial"].is_cuda:
+        res = host.dequantize(cache, length, start, torch.cuda.current_device(), L.stream_handle(cache["K_partial"].device))
+        if res is not None:
+            return res
     bits = cache_bits(cache)
     if bits == 3:
         raise NotImplementedError("dequantize_cache reads INT4 and INT8 caches")
     names = _PLANES[bits]
-    planes = [cache[n] for n in names]
+    planes = _layer_planes(cache, bits)
     kp, vp = cache["K_partial"], cache["V_partial"]
     length, start = int(length), int(start)
     if not 0 <= start <= length:
@@ -221,7 +248,7 @@ def dequantize_cache(cache: dict, length: int, *, start: int = 0, page_size: int
         raise NotImplementedError(f"page_size={page_size}: 64-token pages are taken")
     rest = length % page_size
     done = length - rest
-    if any(t.dim() != 4 for t in planes) or kp.dim() != 4 or kp.shape[:2] != planes[0].shape[:2] or vp.shape != kp.shape:
+    if kp.dim() != 4 or kp.shape[:2] != planes[0].shape[:2] or vp.shape != kp.shape:
         raise ValueError("cache tensors must be one layer's, (B, H_kv, ...)")
     B, H_kv, _, D = kp.shape
     if done > planes[0].shape[2] or done // page_size > planes[1].shape[2] or rest > kp.shape[2]:
