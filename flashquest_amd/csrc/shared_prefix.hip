@@ -55,7 +55,7 @@ struct SharedPart {
     int keys;                            // c.S + t.len
     int rows;                            // rows of an item and KV head
     int items, tiles, splits;            // sequences, row tiles, key splits
-    int pages, per_split;                // pages (the partial one last), pages of a split
+    int pages, per_split;                // pages (the partial one last), pages (row-tile kernel: stages) of a split
     int64_t wgs;                         // items * Hkv * tiles * splits
     float* part;                         // [item][kv head][split][row]: D sums, then all (m, l)
 };
@@ -86,11 +86,15 @@ FQ_DEV void lds_order() { __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
 // Codes as fp16 without a conversion: a code c ORed under an exponent whose last place is
 // 2^-s is 2^(10 - s) + c 2^-s, and the subtraction is exact.  INT4: c / 16, from bits 0..3
 // (64 + c / 16) or bits 4..7 (4 + c / 16) of each half; INT8: c / 256 from bits 0..7 (4 + c / 256).
+FQ_DEV uint32_t opaque_v(uint32_t x) {           // a constant held in a vector register: v_and_or_b32 takes one scalar
+    asm("" : "+v"(x));
+    return x;
+}
 FQ_DEV uint32_t nib_lo(uint32_t w) {
-    return h2_bits(bits_h2((w & 0x000F000Fu) | 0x54005400u) - h2{(_Float16)64.f, (_Float16)64.f});
+    return h2_bits(bits_h2((w & 0x000F000Fu) | opaque_v(0x54005400u)) - h2{(_Float16)64.f, (_Float16)64.f});
 }
 FQ_DEV uint32_t nib_hi(uint32_t w) {
-    return h2_bits(bits_h2((w & 0x00F000F0u) | 0x44004400u) - h2{(_Float16)4.f, (_Float16)4.f});
+    return h2_bits(bits_h2((w & 0x00F000F0u) | opaque_v(0x44004400u)) - h2{(_Float16)4.f, (_Float16)4.f});
 }
 FQ_DEV uint32_t byte_pair(uint32_t w) {          // bytes already at bits 0..7 of each half, 0x44 above them
     return h2_bits(bits_h2(w) - h2{(_Float16)4.f, (_Float16)4.f});
@@ -102,6 +106,154 @@ FQ_DEV float rows_max(float v) {         // over lanes n, n + 16, n + 32, n + 48
     v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
     const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+
+// A row's query as B operands: step s holds channels base + step s .. + 7, in the order the
+// codes unpack (INT4: u, u + 4 side by side).  q times 2^-e with the largest of the row below
+// 1 is exact in fp16 (16-bit inputs: what underflows is below 2^-24 of it); returns the
+// factor from S^T to scores in the log2 domain.
+template <int D, int BITS>
+FQ_DEV float load_query(const uint16_t* q, int base, int step, bool bf, float qk_scale, v8h (&qf)[D / 32]) {
+    float x[D / 32][8];
+    float mx = 0.f;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+        const u32x4 v = *(const u32x4*)(q + base + step * s);
+        const uint32_t d[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            x[s][2 * u] = bf ? bf16_bits_to_f(d[u] & 0xFFFFu) : f16_bits_to_f(d[u] & 0xFFFFu);
+            x[s][2 * u + 1] = bf ? bf16_bits_to_f(d[u] >> 16) : f16_bits_to_f(d[u] >> 16);
+            mx = fmaxf(mx, fmaxf(fabsf(x[s][2 * u]), fabsf(x[s][2 * u + 1])));
+        }
+    }
+    mx = rows_max(mx);
+    const int e = mx > 0.f && mx < INFINITY ? __builtin_amdgcn_frexp_expf(mx) : 0;      // mx = f 2^e, 1/2 <= f < 1
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+        uint32_t d[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int c0 = BITS == 4 ? u : 2 * u, c1 = BITS == 4 ? u + 4 : 2 * u + 1;
+            d[u] = pack_h2(ldexpf(x[s][c0], -e), ldexpf(x[s][c1], -e));
+        }
+        qf[s] = frag(d[0], d[1], d[2], d[3]);
+    }
+    return ldexpf(qk_scale / kKExp, e);
+}
+
+// 8 channels of K codes as fp16 pairs (times 1 / kCodeUp), in the queries' order.
+template <int BITS>
+FQ_DEV void key_codes(const uint32_t* w, uint32_t (&x)[4]) {
+    if constexpr (BITS == 4) {
+        const uint32_t w8 = w[0] >> 8;
+        x[0] = nib_lo(w[0]); x[1] = nib_hi(w[0]); x[2] = nib_lo(w8); x[3] = nib_hi(w8);
+    } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            x[2 * u] = byte_pair(__builtin_amdgcn_perm(0x44444444u, w[u], 0x04010400u));
+            x[2 * u + 1] = byte_pair(__builtin_amdgcn_perm(0x44444444u, w[u], 0x04030402u));
+        }
+    }
+}
+// Channel i of two tokens' V codes (i counted within INT8's dword) as an fp16 pair.
+template <int BITS>
+FQ_DEV uint32_t value_pair(uint32_t wa, uint32_t wb, int i) {
+    const uint32_t y = BITS == 4 ? i >> 1 : i & 3;
+    const uint32_t pr = __builtin_amdgcn_perm(wb, wa, 0x0C000C00u | y | (y + 4) << 16);
+    if constexpr (BITS == 4) return i & 1 ? nib_hi(pr) : nib_lo(pr);
+    else return byte_pair(pr | 0x44004400u);
+}
+// The partial page's bf16: 8 channels of a key, one channel of two tokens.
+template <int BITS>
+FQ_DEV u32x4 tail_keys(const uint16_t* p) {
+    const u32x4 v = *(const u32x4*)p;
+    float x[8];
+    const uint32_t d[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        x[2 * u] = bf16_bits_to_f(d[u] & 0xFFFFu) * kKExp;
+        x[2 * u + 1] = bf16_bits_to_f(d[u] >> 16) * kKExp;
+    }
+    if constexpr (BITS == 4) return u32x4{pack_h2(x[0], x[4]), pack_h2(x[1], x[5]), pack_h2(x[2], x[6]), pack_h2(x[3], x[7])};
+    else return u32x4{pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7])};
+}
+FQ_DEV uint32_t tail_pair(uint32_t wa, uint32_t wb, int odd) {
+    return odd ? pack_h2(bf16_bits_to_f(wa >> 16), bf16_bits_to_f(wb >> 16))
+               : pack_h2(bf16_bits_to_f(wa & 0xFFFFu), bf16_bits_to_f(wb & 0xFFFFu));
+}
+
+// One step of the running softmax over a product's scores s (S^T: a lane's rows are its column's,
+// keys 16 T + 4 lg + r): p = 2^(s rs - reference + kPShift) as the B operands of the second
+// product.  The reference is the largest score seen, but moves only when one exceeds it by 2^8:
+// sums and outputs are then rescaled, until then nothing is.
+template <int QB, int NK, int NT>
+FQ_DEV void softmax_step(v4f (&s)[QB][NK], const float (&rs)[QB], float (&m_run)[QB], v4f (&o)[QB][NT], v4f (&ol)[QB],
+                         v8h (&pb)[QB][NK / 2]) {
+    float ref[QB], mx[QB];
+    bool moved = false;
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        const bool none = m_run[qb] == -INFINITY;
+        ref[qb] = kPShift - (none ? 0.f : m_run[qb]);
+        // exponents before the maximum: products of their own need no canonicalising moves, and
+        // they are final unless the reference moves
+#pragma unroll
+        for (int T = 0; T < NK; ++T)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[qb][T][r] = fmaf(s[qb][T][r], rs[qb], ref[qb]);
+        float m = fmaxf(fmaxf(s[qb][0][0], s[qb][0][1]), s[qb][0][2]);
+        m = fmaxf(m, s[qb][0][3]);
+#pragma unroll
+        for (int T = 1; T < NK; ++T) {
+            m = fmaxf(fmaxf(m, s[qb][T][0]), s[qb][T][1]);
+            m = fmaxf(fmaxf(m, s[qb][T][2]), s[qb][T][3]);
+        }
+        mx[qb] = rows_max(m);
+        moved |= mx[qb] > (none ? -INFINITY : kPShift + kLazy);
+    }
+    if (__builtin_amdgcn_ballot_w64(moved)) {
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+            const float m_new = fmaxf(m_run[qb], mx[qb] - ref[qb]);
+            const float nref = kPShift - (m_new == -INFINITY ? 0.f : m_new);
+            const float al = __builtin_amdgcn_exp2f(m_run[qb] + nref - kPShift), by = nref - ref[qb];
+            m_run[qb] = m_new;
+            ol[qb] *= al;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) o[qb][i] *= al;
+#pragma unroll
+            for (int T = 0; T < NK; ++T)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[qb][T][r] += by;
+        }
+    }
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        uint32_t d[NK][2];
+#pragma unroll
+        for (int T = 0; T < NK; ++T)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+                d[T][r] = pack_h2(__builtin_amdgcn_exp2f(s[qb][T][2 * r]), __builtin_amdgcn_exp2f(s[qb][T][2 * r + 1]));
+#pragma unroll
+        for (int j = 0; j < NK / 2; ++j) pb[qb][j] = frag(d[2 * j][0], d[2 * j][1], d[2 * j + 1][0], d[2 * j + 1][1]);
+    }
+}
+
+// Scores of keys outside lo .. hi, key0 the lane's first.
+template <int QB, int NK>
+FQ_DEV void mask_step(v4f (&s)[QB][NK], int key0, int lo, const int (&hi)[QB]) {
+    asm volatile("");        // keeps the branch round it: most steps mask nothing
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int T = 0; T < NK; ++T)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int key = key0 + 16 * T + r;
+                if (key < lo || key > hi[qb]) s[qb][T][r] = -INFINITY;
+            }
 }
 
 // A page as it is in memory: one lane's K bytes of keys 16 T + n (channels D/4 lg ..) and V
@@ -166,34 +318,8 @@ __global__ __launch_bounds__(64 * kW) void shared_attn_kernel(SharedParams a) {
         const int row = min(row0 + 16 * qb + n, P.rows - 1);
         const int g = row % a.G, i = (row / a.G) % a.Sq, b = pi == 1 ? item : row / (a.G * a.Sq);
         hi[qb] = pi == 1 ? P.keys - a.Sq + i : P.keys - 1;
-        const uint16_t* q = (const uint16_t*)a.q + b * a.q_s[0] + (int64_t)(h * a.G + g) * a.q_s[1] + i * a.q_s[2] +
-                            (D / 4) * lg;
-        float x[NS][8];
-        float mx = 0.f;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            const u32x4 v = *(const u32x4*)(q + 8 * s);
-            const uint32_t d[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                x[s][2 * u] = a.bf16 ? bf16_bits_to_f(d[u] & 0xFFFFu) : f16_bits_to_f(d[u] & 0xFFFFu);
-                x[s][2 * u + 1] = a.bf16 ? bf16_bits_to_f(d[u] >> 16) : f16_bits_to_f(d[u] >> 16);
-                mx = fmaxf(mx, fmaxf(fabsf(x[s][2 * u]), fabsf(x[s][2 * u + 1])));
-            }
-        }
-        mx = rows_max(mx);
-        const int e = mx > 0.f && mx < INFINITY ? __builtin_amdgcn_frexp_expf(mx) : 0;      // mx = f 2^e, 1/2 <= f < 1
-        rs[qb] = ldexpf(a.qk_scale / kKExp, e);
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            uint32_t d[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {        // INT4: channels in the order the codes unpack
-                const int c0 = BITS == 4 ? u : 2 * u, c1 = BITS == 4 ? u + 4 : 2 * u + 1;
-                d[u] = pack_h2(ldexpf(x[s][c0], -e), ldexpf(x[s][c1], -e));
-            }
-            qf[qb][s] = frag(d[0], d[1], d[2], d[3]);
-        }
+        const uint16_t* q = (const uint16_t*)a.q + b * a.q_s[0] + (int64_t)(h * a.G + g) * a.q_s[1] + i * a.q_s[2];
+        rs[qb] = load_query<D, BITS>(q, (D / 4) * lg, 8, a.bf16, a.qk_scale, qf[qb]);
     }
 
     v4f o[QB][NT], ol[QB];
@@ -222,53 +348,9 @@ __global__ __launch_bounds__(64 * kW) void shared_attn_kernel(SharedParams a) {
                 for (int qb = 0; qb < QB; ++qb) s[qb][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[qb][st], s[qb][T], 0, 0, 0);
             }
         }
-        if (masked) {
-            const int k0 = page * kPg + 4 * lg;
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb)
-#pragma unroll
-                for (int T = 0; T < 4; ++T)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int key = k0 + 16 * T + r;
-                        if (key < lo || key > hi[qb]) s[qb][T][r] = -INFINITY;
-                    }
-        }
-        float mx[QB];
-        bool moved = false;
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) {
-            float t[4];
-#pragma unroll
-            for (int T = 0; T < 4; ++T) t[T] = fmaxf(fmaxf(s[qb][T][0], s[qb][T][1]), fmaxf(s[qb][T][2], s[qb][T][3]));
-            mx[qb] = rows_max(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]))) * rs[qb];
-            moved |= mx[qb] > m_run[qb] + kLazy;
-        }
-        if (__builtin_amdgcn_ballot_w64(moved)) {
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb) {
-                const float m_new = fmaxf(m_run[qb], mx[qb]);
-                const float al = __builtin_amdgcn_exp2f(m_run[qb] - (m_new == -INFINITY ? 0.f : m_new));
-                m_run[qb] = m_new;
-                ol[qb] *= al;
-#pragma unroll
-                for (int i = 0; i < NT; ++i) o[qb][i] *= al;
-            }
-        }
+        if (masked) mask_step(s, page * kPg + 4 * lg, lo, hi);
         v8h pb[QB][2];
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) {
-            const float ref = kPShift - (m_run[qb] == -INFINITY ? 0.f : m_run[qb]);
-            uint32_t d[4][2];
-#pragma unroll
-            for (int T = 0; T < 4; ++T)
-#pragma unroll
-                for (int r = 0; r < 2; ++r)
-                    d[T][r] = pack_h2(__builtin_amdgcn_exp2f(fmaf(s[qb][T][2 * r], rs[qb], ref)),
-                                      __builtin_amdgcn_exp2f(fmaf(s[qb][T][2 * r + 1], rs[qb], ref)));
-            pb[qb][0] = frag(d[0][0], d[0][1], d[1][0], d[1][1]);
-            pb[qb][1] = frag(d[2][0], d[2][1], d[3][0], d[3][1]);
-        }
+        softmax_step(s, rs, m_run, o, ol, pb);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -368,17 +450,7 @@ __global__ __launch_bounds__(64 * kW) void shared_attn_kernel(SharedParams a) {
             }
         auto kf = [&](int T, int s) {
             uint32_t x[4];
-            if constexpr (BITS == 4) {
-                const uint32_t wd = r.k[T][s], w8 = wd >> 8;
-                x[0] = nib_lo(wd); x[1] = nib_hi(wd); x[2] = nib_lo(w8); x[3] = nib_hi(w8);
-            } else {
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint32_t wd = r.k[T][2 * s + u];
-                    x[2 * u] = byte_pair(__builtin_amdgcn_perm(0x44444444u, wd, 0x04010400u));
-                    x[2 * u + 1] = byte_pair(__builtin_amdgcn_perm(0x44444444u, wd, 0x04030402u));
-                }
-            }
+            key_codes<BITS>(&r.k[T][BITS == 4 ? s : 2 * s], x);
             return frag(fma_h2(x[0], sk[s].x, mk[s].x), fma_h2(x[1], sk[s].y, mk[s].y), fma_h2(x[2], sk[s].z, mk[s].z),
                         fma_h2(x[3], sk[s].w, mk[s].w));
         };
@@ -386,15 +458,8 @@ __global__ __launch_bounds__(64 * kW) void shared_attn_kernel(SharedParams a) {
             uint32_t x[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {                // keys 2u, 2u + 1 of the slots
-                const uint32_t wa = r.v[8 * j + 2 * u][BITS == 8 ? i >> 2 : 0], wb = r.v[8 * j + 2 * u + 1][BITS == 8 ? i >> 2 : 0];
-                const uint32_t y = BITS == 4 ? i >> 1 : i & 3;
-                if constexpr (BITS == 4) {
-                    const uint32_t pr = __builtin_amdgcn_perm(wb, wa, 0x0C000C00u | y | (y + 4) << 16);
-                    x[u] = i & 1 ? nib_hi(pr) : nib_lo(pr);
-                } else {
-                    const uint32_t pr = __builtin_amdgcn_perm(wb, wa, 0x0C000C00u | y | (y + 4) << 16);
-                    x[u] = byte_pair(pr | 0x44004400u);
-                }
+                const int d = BITS == 8 ? i >> 2 : 0;
+                x[u] = value_pair<BITS>(r.v[8 * j + 2 * u][d], r.v[8 * j + 2 * u + 1][d], i);
             }
             return frag(fma_h2(x[0], sv[j][0].x, mv[j][0].x), fma_h2(x[1], sv[j][0].y, mv[j][0].y),
                         fma_h2(x[2], sv[j][1].x, mv[j][1].x), fma_h2(x[3], sv[j][1].y, mv[j][1].y));
@@ -408,16 +473,7 @@ __global__ __launch_bounds__(64 * kW) void shared_attn_kernel(SharedParams a) {
         const uint16_t* kt = (const uint16_t*)t.k + item * t.ks[1] + h * t.ks[2] + (D / 4) * lg;
         const uint16_t* vt = (const uint16_t*)t.v + item * t.vs[1] + h * t.vs[2] + (D / 16) * n;
         auto kf = [&](int T, int s) {
-            const u32x4 v = *(const u32x4*)(kt + (int64_t)min(16 * T + n, t.len - 1) * t.ks[3] + 8 * s);
-            float x[8];
-            const uint32_t d[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                x[2 * u] = bf16_bits_to_f(d[u] & 0xFFFFu) * kKExp;
-                x[2 * u + 1] = bf16_bits_to_f(d[u] >> 16) * kKExp;
-            }
-            if constexpr (BITS == 4) return frag(pack_h2(x[0], x[4]), pack_h2(x[1], x[5]), pack_h2(x[2], x[6]), pack_h2(x[3], x[7]));
-            else return frag(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]));
+            return __builtin_bit_cast(v8h, tail_keys<BITS>(kt + (int64_t)min(16 * T + n, t.len - 1) * t.ks[3] + 8 * s));
         };
         uint32_t tv[16][NT / 2];
 #pragma unroll
@@ -437,9 +493,7 @@ __global__ __launch_bounds__(64 * kW) void shared_attn_kernel(SharedParams a) {
             uint32_t x[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const uint32_t wa = tv[8 * j + 2 * u][i >> 1], wb = tv[8 * j + 2 * u + 1][i >> 1];
-                x[u] = i & 1 ? pack_h2(bf16_bits_to_f(wa >> 16), bf16_bits_to_f(wb >> 16))
-                             : pack_h2(bf16_bits_to_f(wa & 0xFFFFu), bf16_bits_to_f(wb & 0xFFFFu));
+                x[u] = tail_pair(tv[8 * j + 2 * u][i >> 1], tv[8 * j + 2 * u + 1][i >> 1], i & 1);
             }
             return frag(x[0], x[1], x[2], x[3]);
         };
@@ -522,6 +576,365 @@ __global__ __launch_bounds__(64 * kW) void shared_attn_kernel(SharedParams a) {
     }
 }
 
+// ---- many rows: keys and values staged in LDS ------------------------------------------
+// With more rows than a wave or two take, turning a page into operands once per 32 rows is
+// what the time goes into.  Here a workgroup of 8 waves turns each stage of 128 keys (two
+// pages) into fp16 once, K as [key][channel] and V as [channel][key] in LDS, while the stage
+// before is attended: 256 / KG rows (32 a wave) times KG groups of keys, key group kg taking
+// keys 128 kg / KG .. of every stage for its rows; the groups' states meet in LDS at the end.
+// The codes of stage t + 2 are loaded before stage t + 1 is written: no wait on memory in
+// the loop but the one for loads that are a stage old.
+//
+// LDS holds a plane for each lane group lg of the operands: K's plane has a row per key of the
+// chunks (8 channels, 16 bytes) 4 st + lg, V's a row per channel of the chunks (8 keys) 4 jb + lg.
+// A 16-byte read of 64 lanes is served 16 lanes at a time, 8 of one lg and the other 8 n of the
+// next; with chunk x of row r at x ^ (r / rows of 256 bytes) those 16 hit all banks once, and so
+// do the writes (planes 64 bytes apart modulo 256; not for K with D = 64, 4 on a bank).  V's
+// channels are dealt to the tiles as the codes unpack (tile i: channels D/16 n + i), so that the
+// 16 lanes that write channel i of their codes write neighbouring rows.
+constexpr int kTW = 8;                   // waves
+constexpr int kST = 128;                 // keys of a stage
+// Scheduling groups: n LDS reads, then (m matrix instructions, one read) until the reads are out,
+// then the rest: operand reads stay n ahead of their use (left alone, the scheduler puts each
+// right before it and every pair of matrix instructions waits for LDS).
+template <int READS, int AHEAD, int MFMA_PER_READ>
+FQ_DEV void reads_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < READS - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, MFMA_PER_READ, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * MFMA_PER_READ, 0);
+}
+template <int D> struct StageLds {
+    static constexpr int NS = D / 32;
+    static constexpr int KROW = 16 * NS, KPL = kST * KROW + (D == 128 ? 64 : 0), KB = 4 * KPL;
+    static constexpr int VROW = 64, VPL = D * VROW + 64, VB = 4 * VPL;
+    FQ_DEV static int k_at(int lg, int key, int st) { return lg * KPL + key * KROW + 16 * (st ^ ((key / (16 / NS)) & (NS - 1))); }
+    FQ_DEV static int v_at(int lg, int row, int jb) { return lg * VPL + row * VROW + 16 * (jb ^ ((row >> 2) & 3)); }
+};
+
+template <int D, int BITS, typename MT, int KG>
+__global__ __launch_bounds__(64 * kTW) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void shared_tile_kernel(SharedParams a) {
+    constexpr int QB = 2, NS = D / 32, NT = D / 16, VC = D / 16;
+    constexpr int RG = kTW / KG;                 // row groups
+    constexpr int RT = 32 * RG;                  // rows of the workgroup
+    constexpr int SUB = KG == 4 ? 32 : 64;       // keys of a wave's product
+    constexpr int NK = SUB / 16, NJ = SUB / 32, NSUB = kST / KG / SUB;       // 16-key tiles, 32-key steps, products a stage
+    constexpr int CPR = D / 8, KPT = D / 32;     // K: chunks of a row, rows a thread turns
+    constexpr int KW = BITS / 4, VW = VC * BITS / 8 == 8 ? 2 : 1;            // dwords of 8 K channels, of VC V channels
+    constexpr int AHEAD = 6;                     // operand reads in flight
+    using Lds = StageLds<D>;
+    __shared__ __attribute__((aligned(16))) uint8_t s_k[2][Lds::KB];
+    __shared__ __attribute__((aligned(16))) uint8_t s_v[2][Lds::VB];
+    const int tid = threadIdx.x, L = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_id());
+    const int n = L & 15, lg = L >> 4;
+
+    int64_t blk = blockIdx.x;
+    const int pi = a.first < a.last && blk >= a.p[0].wgs ? 1 : a.first;
+    if (pi > a.first) blk -= a.p[0].wgs;
+    const SharedPart& P = a.p[pi];
+    const int h = (int)(blk % a.Hkv);
+    const int64_t r1 = blk / a.Hkv;
+    const int tile = (int)(r1 % P.tiles);
+    const int64_t r2 = r1 / P.tiles;
+    const int split = (int)(r2 % P.splits), item = (int)(r2 / P.splits);
+    const Int4Cache& c = P.c;
+    const int code_pages = c.S / kPg;
+    const int kg = w / RG;                       // key group
+    const int wg_row0 = tile * RT, row0 = wg_row0 + (w % RG) * 32;
+    const bool wave_on = row0 < P.rows;
+
+    int hi[QB], lo = 0, hi_all = P.keys - 1;
+    float rs[QB];
+    v8h qf[QB][NS];
+    if (pi == 1) {
+        if (a.start) lo = min(max(a.start[item], 0), P.keys);
+        hi_all = P.keys - a.Sq + min(row0, P.rows - 1) / a.G;
+    }
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        const int row = min(row0 + 16 * qb + n, P.rows - 1);
+        const int g = row % a.G, i = (row / a.G) % a.Sq, b = pi == 1 ? item : row / (a.G * a.Sq);
+        hi[qb] = pi == 1 ? P.keys - a.Sq + i : P.keys - 1;
+        const uint16_t* q = (const uint16_t*)a.q + b * a.q_s[0] + (int64_t)(h * a.G + g) * a.q_s[1] + i * a.q_s[2];
+        rs[qb] = load_query<D, BITS>(q, 8 * lg, 32, a.bf16, a.qk_scale, qf[qb]);
+    }
+
+    v4f o[QB][NT], ol[QB];
+    float m_run[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        m_run[qb] = -INFINITY;
+        ol[qb] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NT; ++i) o[qb][i] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    const v8h ones = frag(0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u);
+
+    // This thread's part of a stage: KPT keys' 8 channels of K and 4 keys' VC channels of V, of
+    // page 2 t + pg (a wave's threads are in one page).
+    const int pg = w >> 2;
+    const int kc = tid % CPR, kr = (tid & 255) / CPR;              // K: chunk, first row in the page
+    // V: channels VC vc .., keys 4 vq .. in the page (a wave's four vq fill whole 16-byte chunks)
+    const int vt = (tid >> 4) & 15, vc = tid & 15, vq = (vt & 8) | (vt & 1) << 2 | ((vt >> 1) & 3);
+    const uint8_t* kb = c.kp + item * c.kp_s[1] + h * c.kp_s[2] + kr * c.kp_s[3] + kc * BITS;
+    const uint8_t* vb = c.vp + item * c.vp_s[1] + h * c.vp_s[2] + 4 * vq * c.vp_s[3] + vc * (VC * BITS / 8);
+    const uint16_t* ksb = (const uint16_t*)c.ksc + item * c.ksc_s[1] + h * c.ksc_s[2] + 8 * kc;
+    const uint16_t* kmb = (const uint16_t*)c.kmn + item * c.kmn_s[1] + h * c.kmn_s[2] + 8 * kc;
+    const int vg = vc * c.G >> 4;
+    const uint16_t* vsb = (const uint16_t*)c.vsc + item * c.vsc_s[1] + h * c.vsc_s[2] + 4 * vq * c.vsc_s[3] + vg;
+    const uint16_t* vmb = (const uint16_t*)c.vmn + item * c.vmn_s[1] + h * c.vmn_s[2] + 4 * vq * c.vmn_s[3] + vg;
+    struct Raw {
+        uint32_t k[KPT][KW], v[4][VW];
+        u32x4 ks, km;
+        uint32_t vs[4], vm[4];
+    };
+    auto load = [&](Raw& r, int t) __attribute__((always_inline)) {             // code pages; others are read when they are written
+        const int page = min(2 * t + pg, code_pages - 1);
+        if (page < 0) return;
+        const int64_t t0 = (int64_t)page * kPg;
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) {
+            const uint8_t* p = kb + (t0 + 256 / CPR * j) * c.kp_s[3];
+            if constexpr (KW == 1) r.k[j][0] = *(const uint32_t*)p;
+            else { const u32x2 x = *(const u32x2*)p; r.k[j][0] = x.x; r.k[j][1] = x.y; }
+        }
+        r.ks = *(const u32x4*)(ksb + page * c.ksc_s[3]);
+        r.km = *(const u32x4*)(kmb + page * c.kmn_s[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint8_t* p = vb + (t0 + j) * c.vp_s[3];
+            if constexpr (VC * BITS == 16) r.v[j][0] = *(const uint16_t*)p;
+            else if constexpr (VW == 1) r.v[j][0] = *(const uint32_t*)p;
+            else { const u32x2 x = *(const u32x2*)p; r.v[j][0] = x.x; r.v[j][1] = x.y; }
+            r.vs[j] = vsb[(t0 + j) * c.vsc_s[3]];
+            r.vm[j] = vmb[(t0 + j) * c.vmn_s[3]];
+        }
+    };
+    auto put_k = [&](int buf, int j, u32x4 x) __attribute__((always_inline)) {
+        const int row = kPg * pg + kr + 256 / CPR * j;
+        *(u32x4*)&s_k[buf][Lds::k_at(kc & 3, row, kc >> 2)] = x;
+    };
+    const int vjb = 2 * pg + (vq >> 3), vlg = vq & 3, vhalf = 8 * ((vq >> 2) & 1);
+    auto put_v = [&](int buf, int i, u32x2 x) __attribute__((always_inline)) {
+        *(u32x2*)&s_v[buf][Lds::v_at(vlg, 16 * i + vc, vjb) + vhalf] = x;
+    };
+    auto write = [&](const Raw& r, int t, int buf) __attribute__((always_inline)) {
+        const int page = 2 * t + pg;
+        if (page < code_pages) {
+            constexpr float up = kCodeUp<BITS>;
+            uint32_t sk[4], mk[4];
+            const uint32_t sw[4] = {r.ks.x, r.ks.y, r.ks.z, r.ks.w}, mw[4] = {r.km.x, r.km.y, r.km.z, r.km.w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {        // channels u and u + 4 (INT4), 2 u and 2 u + 1 (INT8)
+                const int c0 = BITS == 4 ? u : 2 * u, c1 = BITS == 4 ? u + 4 : 2 * u + 1;
+                sk[u] = pack_h2(meta_f<MT>(sw[c0 >> 1] >> (16 * (c0 & 1))) * (up * kKExp), meta_f<MT>(sw[c1 >> 1] >> (16 * (c1 & 1))) * (up * kKExp));
+                mk[u] = pack_h2(meta_f<MT>(mw[c0 >> 1] >> (16 * (c0 & 1))) * kKExp, meta_f<MT>(mw[c1 >> 1] >> (16 * (c1 & 1))) * kKExp);
+            }
+#pragma unroll
+            for (int j = 0; j < KPT; ++j) {
+                uint32_t x[4];
+                key_codes<BITS>(&r.k[j][0], x);
+                put_k(buf, j, u32x4{fma_h2(x[0], sk[0], mk[0]), fma_h2(x[1], sk[1], mk[1]), fma_h2(x[2], sk[2], mk[2]), fma_h2(x[3], sk[3], mk[3])});
+            }
+            uint32_t sv[2], mv[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                sv[u] = pack_h2(meta_f<MT>(r.vs[2 * u]) * up, meta_f<MT>(r.vs[2 * u + 1]) * up);
+                mv[u] = pack_h2(meta_f<MT>(r.vm[2 * u]), meta_f<MT>(r.vm[2 * u + 1]));
+            }
+            if (page * kPg < lo) {               // values of padding tokens count as 0, whatever they are
+                asm volatile("");
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int key = page * kPg + 4 * vq + 2 * u;
+                    const uint32_t on = (key >= lo ? 0xFFFFu : 0u) | (key + 1 >= lo ? 0xFFFF0000u : 0u);
+                    sv[u] &= on;
+                    mv[u] &= on;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < VC; ++i) {
+                const int d = BITS == 8 ? i >> 2 : 0;
+                put_v(buf, i, u32x2{fma_h2(value_pair<BITS>(r.v[0][d], r.v[1][d], i), sv[0], mv[0]),
+                                    fma_h2(value_pair<BITS>(r.v[2][d], r.v[3][d], i), sv[1], mv[1])});
+            }
+        } else if (page * kPg < P.keys) {        // the partial page
+            const TailArgs& tl = P.t;
+            const uint16_t* kt = (const uint16_t*)tl.k + item * tl.ks[1] + h * tl.ks[2] + 8 * kc;
+            const uint16_t* vt = (const uint16_t*)tl.v + item * tl.vs[1] + h * tl.vs[2] + VC * vc;
+#pragma unroll
+            for (int j = 0; j < KPT; ++j)
+                put_k(buf, j, tail_keys<BITS>(kt + (int64_t)min(kr + 256 / CPR * j, tl.len - 1) * tl.ks[3]));
+            uint32_t x[4][VC / 2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = 4 * vq + j;
+                const bool on = key < tl.len && page * kPg + key >= lo;
+                const uint32_t* p = (const uint32_t*)(vt + (int64_t)min(key, tl.len - 1) * tl.vs[3]);
+#pragma unroll
+                for (int u = 0; u < VC / 2; ++u) x[j][u] = on ? p[u] : 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < VC; ++i)
+                put_v(buf, i, u32x2{tail_pair(x[0][i >> 1], x[1][i >> 1], i & 1), tail_pair(x[2][i >> 1], x[3][i >> 1], i & 1)});
+        } else {                                 // no keys: masked, and values of 0
+#pragma unroll
+            for (int j = 0; j < KPT; ++j) put_k(buf, j, u32x4{0u, 0u, 0u, 0u});
+#pragma unroll
+            for (int i = 0; i < VC; ++i) put_v(buf, i, u32x2{0u, 0u});
+        }
+    };
+
+    // Operand addresses of the lane: row n (rows 16 apart are a constant apart).
+    int k_lane[NS];
+#pragma unroll
+    for (int st = 0; st < NS; ++st) k_lane[st] = Lds::k_at(lg, n, st);
+    const int v_lane = Lds::v_at(lg, n, 0);      // its chunk bits XORed with the key block's
+    static_assert(Lds::VPL % 64 == 0 && Lds::VROW == 64, "chunk bits are the low ones of a row");
+
+    // The two products of a wave's SUB keys from key `k0` of a stage on.
+    auto qk = [&](const uint8_t* sk, int k0, v4f (&s)[QB][NK]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) s[qb][kb] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < NS; ++st)
+#pragma unroll
+            for (int kb = 0; kb < NK; ++kb) {
+                const v8h k = *(const v8h*)(sk + k_lane[st] + (k0 + 16 * kb) * Lds::KROW);
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) s[qb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[qb][st], s[qb][kb], 0, 0, 0);
+            }
+        reads_ahead<NS * NK, AHEAD, QB>();
+    };
+    auto pv = [&](const uint8_t* sv, int k0, const v8h (&pb)[QB][NJ]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const v8h v = *(const v8h*)(sv + (v_lane ^ 16 * (k0 / 32 + j)) + 16 * i * Lds::VROW);
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pb[qb][j], o[qb][i], 0, 0, 0);
+            }
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) ol[qb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pb[qb][j], ol[qb], 0, 0, 0);
+        }
+        reads_ahead<NT * NJ, AHEAD, QB>();
+        __builtin_amdgcn_sched_group_barrier(0x008, QB * NJ, 0);
+    };
+
+    // Stages of this workgroup: those of its split with keys between the first and the last
+    // row's last.
+    const int hi_top = pi == 1 ? P.keys - a.Sq + min(wg_row0 + RT - 1, P.rows - 1) / a.G : P.keys - 1;
+    const int t_begin = max(split * P.per_split, lo / kST);
+    const int t_end = min(min((split + 1) * P.per_split, (P.pages + 1) / 2), hi_top / kST + 1);
+    if (t_begin < t_end) {
+        Raw raw;
+        load(raw, t_begin);
+        write(raw, t_begin, 0);
+        if (t_begin + 1 < t_end) load(raw, t_begin + 1);
+        lds_barrier();
+        for (int t = t_begin; t < t_end; ++t) {
+            const int buf = (t - t_begin) & 1;
+            auto next = [&]() __attribute__((always_inline)) {
+                if (t + 1 >= t_end) return;
+                write(raw, t + 1, buf ^ 1);
+                if (t + 2 < t_end) load(raw, t + 2);
+            };
+            // a SIMD's two waves (w, w + 4) take their vector-only part at opposite ends of the stage
+            if (w >= kTW / 2) next();
+            if (wave_on) {
+                const int k0 = kg * (kST / KG);
+                v8h pb[QB][NJ];
+#pragma unroll 1
+                for (int u = 0; u < NSUB; ++u) {
+                    v4f s[QB][NK];
+                    qk(s_k[buf], k0 + SUB * u, s);
+                    const int key0 = t * kST + k0 + SUB * u;
+                    if (key0 < lo || key0 + SUB - 1 > hi_all) mask_step(s, key0 + 4 * lg, lo, hi);
+                    softmax_step(s, rs, m_run, o, ol, pb);
+                    __builtin_amdgcn_sched_barrier(0);
+                    pv(s_v[buf], k0 + SUB * u, pb);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if (w < kTW / 2) next();
+            lds_barrier();
+        }
+    }
+
+    // The key groups' states of a row group meet in key group 0's wave.
+    if constexpr (KG > 1) {
+        constexpr int NSL = QB * NT, kHalf = 2 * kST * D * 2 / 16;       // of each of the K and V buffers
+        static_assert((kTW - RG) * NSL * 64 * 16 <= 2 * kHalf * 16, "states fit the stage buffers");
+        __shared__ float2 s_ml[(kTW - RG) * QB * 64];
+        v4f* st0 = (v4f*)&s_k[0][0];
+        v4f* st1 = (v4f*)&s_v[0][0];
+        auto slot = [&](int i) -> v4f* { return i < kHalf ? st0 + i : st1 + (i - kHalf); };
+        if (kg > 0) {
+            const int src = w - RG;
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) *slot((src * NSL + qb * NT + i) * 64 + L) = o[qb][i];
+                s_ml[(src * QB + qb) * 64 + L] = make_float2(m_run[qb], ol[qb][0]);
+            }
+        }
+        __syncthreads();
+        if (kg > 0) return;
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+            float m[KG], l[KG], mm = m_run[qb];
+            m[0] = m_run[qb]; l[0] = ol[qb][0];
+#pragma unroll
+            for (int u = 1; u < KG; ++u) {
+                const float2 x = s_ml[(((u - 1) * RG + w) * QB + qb) * 64 + L];
+                m[u] = x.x; l[u] = x.y;
+                mm = fmaxf(mm, m[u]);
+            }
+            const float mu = mm == -INFINITY ? 0.f : mm;
+            float wt[KG], ls = 0.f;
+#pragma unroll
+            for (int u = 0; u < KG; ++u) {
+                wt[u] = __builtin_amdgcn_exp2f(m[u] - mu);
+                ls = fmaf(wt[u], l[u], ls);
+            }
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                v4f t = o[qb][i] * wt[0];
+#pragma unroll
+                for (int u = 1; u < KG; ++u) {
+                    const v4f y = *slot((((u - 1) * RG + w) * NSL + qb * NT + i) * 64 + L);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) t[r] = fmaf(wt[u], y[r], t[r]);
+                }
+                o[qb][i] = t;
+            }
+            m_run[qb] = mm;
+            ol[qb][0] = ls;
+        }
+    }
+    const int64_t base = ((int64_t)(item * a.Hkv + h) * P.splits + split) * P.rows;
+    const int64_t all = (int64_t)P.items * a.Hkv * P.splits * P.rows;
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        const int row = row0 + 16 * qb + n;
+        if (row >= P.rows) continue;
+        float* dst = P.part + (base + row) * D + (D / 4) * lg;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)              // channels D/16 (4 lg + r) + i
+#pragma unroll
+            for (int i = 0; i < NT; i += 4)
+                *(v4f*)(dst + NT * r + i) = v4f{o[qb][i][r], o[qb][i + 1][r], o[qb][i + 2][r], o[qb][i + 3][r]};
+        if (lg == 0) *(float2*)(P.part + all * D + 2 * (base + row)) = make_float2(m_run[qb], ol[qb][0]);
+    }
+}
+
 // Joins the shares of a row: prefix splits, then suffix splits, in order.  D/4 lanes a row,
 // four channels a lane.
 template <int D>
@@ -585,22 +998,33 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams a) 
             l == 0.f ? -INFINITY : (M - kPShift + __log2f(l)) * kLn2;
 }
 
-// Rows a wave takes: 16 where they hold an item's rows, else 32.
-int row_blocks(int rows) { return rows <= 16 ? 1 : 2; }
+// How a part's rows are taken: 16 or 32 rows a wave (nb 1, 2: shared_attn_kernel), or 256 / kg
+// rows a workgroup over stages in LDS (kg 1, 2, 4: shared_tile_kernel).
+struct Form { int nb, kg; };
 
-// Key splits of a part: enough workgroups for the GPU's slots, at least 4 pages (one a wave) each.
-void plan_part(SharedPart& p, int Hkv, int qb) {
-    const int slots = 512;
-    p.tiles = (p.rows + 16 * qb - 1) / (16 * qb);
-    p.pages = (p.keys + kPg - 1) / kPg;
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Tiles and key splits of a part under a form: splits are chosen so that the workgroups fill
+// the GPU's slots once or a few times evenly.
+void plan_part(SharedPart& p, int Hkv, const Form& f) {
+    const bool tile = f.kg > 0;
+    const int slots = tile ? 256 : 512;
+    const int rt = tile ? 256 / f.kg : 16 * f.nb;
+    p.tiles = (int)ceil_div(p.rows, rt);
+    p.pages = (int)ceil_div(p.keys, kPg);
+    const int units = tile ? (int)ceil_div(p.pages, 2) : p.pages;
     const int64_t groups = (int64_t)p.items * Hkv * p.tiles;
-    const int most = std::max(1, (p.pages + kW - 1) / kW);
+    const int most = std::max<int>(1, (int)(tile ? ceil_div(units, 2) : ceil_div(units, kW)));
     int64_t s = std::max<int64_t>(1, slots / std::max<int64_t>(1, groups));
     s = std::min<int64_t>(s, most);
-    p.per_split = (int)((p.pages + s - 1) / s);
-    if (p.per_split < 1) p.per_split = 1;
-    p.splits = std::max(1, (p.pages + p.per_split - 1) / p.per_split);
+    p.per_split = std::max(1, (int)ceil_div(units, s));
+    p.splits = std::max(1, (int)ceil_div(units, p.per_split));
     p.wgs = groups * p.splits;
+}
+
+Form form_of(int rows) {
+    if (rows <= 16) return {1, 0};
+    return {2, rows <= 64 ? 4 : rows <= 128 ? 2 : 1};
 }
 
 size_t part_floats(const SharedPart& p, int Hkv, int D) {
@@ -617,10 +1041,10 @@ hipError_t launch_shared_prefix(const Int4Cache& pc, const TailArgs& pt, const I
     const int G = q.H_q / pc.Hkv;
     a.p[0].c = pc; a.p[0].t = pt; a.p[0].keys = pc.S + pt.len; a.p[0].items = 1; a.p[0].rows = q.B * q.S_q * G;
     a.p[1].c = sc; a.p[1].t = st_; a.p[1].keys = sc.S + st_.len; a.p[1].items = q.B; a.p[1].rows = q.S_q * G;
-    int qb[2];
+    Form f[2];
     for (int i = 0; i < 2; ++i) {
-        qb[i] = row_blocks(a.p[i].rows);
-        plan_part(a.p[i], pc.Hkv, qb[i]);
+        f[i] = form_of(a.p[i].rows);
+        plan_part(a.p[i], pc.Hkv, f[i]);
     }
     if (!ws) {
         *bytes = (part_floats(a.p[0], pc.Hkv, pc.D) + part_floats(a.p[1], pc.Hkv, pc.D)) * sizeof(float);
@@ -634,30 +1058,37 @@ hipError_t launch_shared_prefix(const Int4Cache& pc, const TailArgs& pt, const I
     a.bf16 = q.dtype == FQ_BF16;
     a.B = q.B; a.Hq = q.H_q; a.Hkv = pc.Hkv; a.G = G; a.Sq = q.S_q;
     a.qk_scale = qk_scale;
-    auto attend = [&](int first, int last, int nb) {
+    auto attend = [&](int first, int last, const Form& f) {
         a.first = first; a.last = last;
         int64_t wgs = 0;
         for (int i = first; i <= last; ++i) wgs += a.p[i].wgs;
         const dim3 grid((unsigned)wgs);
         const bool bf = pc.meta_dtype == FQ_BF16;
 #define FQ_SP(D_, B_, Q_)                                                                                              \
-    if (pc.D == D_ && pc.bits == B_ && nb == Q_) {                                                                     \
-        if (bf) hipLaunchKernelGGL((shared_attn_kernel<D_, B_, struct bf16, Q_>), grid, dim3(64 * kW), 0, st, a);      \
+    if (pc.D == D_ && pc.bits == B_ && f.kg == 0 && f.nb == Q_) {                                                      \
+        if (bf) hipLaunchKernelGGL((shared_attn_kernel<D_, B_, bf16, Q_>), grid, dim3(64 * kW), 0, st, a);             \
         else hipLaunchKernelGGL((shared_attn_kernel<D_, B_, f16, Q_>), grid, dim3(64 * kW), 0, st, a);                 \
         return hipGetLastError();                                                                                      \
     }
-#define FQ_SPQ(D_, B_) FQ_SP(D_, B_, 1) FQ_SP(D_, B_, 2)
+#define FQ_ST(D_, B_, K_)                                                                                              \
+    if (pc.D == D_ && pc.bits == B_ && f.kg == K_) {                                                                   \
+        if (bf) hipLaunchKernelGGL((shared_tile_kernel<D_, B_, bf16, K_>), grid, dim3(64 * kTW), 0, st, a);            \
+        else hipLaunchKernelGGL((shared_tile_kernel<D_, B_, f16, K_>), grid, dim3(64 * kTW), 0, st, a);                \
+        return hipGetLastError();                                                                                      \
+    }
+#define FQ_SPQ(D_, B_) FQ_SP(D_, B_, 1) FQ_SP(D_, B_, 2) FQ_ST(D_, B_, 1) FQ_ST(D_, B_, 2) FQ_ST(D_, B_, 4)
         FQ_SPQ(128, 4) FQ_SPQ(128, 8) FQ_SPQ(64, 4) FQ_SPQ(64, 8)
 #undef FQ_SPQ
+#undef FQ_ST
 #undef FQ_SP
         return hipErrorInvalidValue;
     };
     hipError_t e;
-    if (qb[0] == qb[1]) {
-        e = attend(0, 1, qb[0]);
+    if (f[0].kg == f[1].kg && (f[0].kg > 0 || f[0].nb == f[1].nb)) {
+        e = attend(0, 1, f[0]);
     } else {
-        e = attend(0, 0, qb[0]);
-        if (e == hipSuccess) e = attend(1, 1, qb[1]);
+        e = attend(0, 0, f[0]);
+        if (e == hipSuccess) e = attend(1, 1, f[1]);
     }
     if (e != hipSuccess) return e;
     const int64_t threads = (int64_t)q.B * q.H_q * q.S_q * (pc.D / 4);
