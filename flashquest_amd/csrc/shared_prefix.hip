@@ -278,8 +278,10 @@ struct alignas(16) WaveMeta {
 // The keys of a lane's k-slots of step j of the second product: 32 j + 4 lg + {0..3}, then + 16.
 FQ_DEV constexpr int slot_key(int u) { return (u & 3) + 16 * (u >> 2); }      // u = 0 .. 7, before 32 j + 4 lg
 
-template <int D, int BITS, typename MT, int QB>
-__global__ __launch_bounds__(64 * kW) void shared_attn_kernel(SharedParams a) {
+template <int D, int BITS, typename MT>
+__global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void shared_attn_kernel(SharedParams a) {
+    constexpr int QB = 1;
     constexpr int NS = D / 32, NT = D / 16, RT = 16 * QB;
     constexpr int KB = D * BITS / 32;            // bytes of a lane's D/4 channels
     __shared__ WaveMeta<D> s_meta[kW];
@@ -508,16 +510,13 @@ __global__ __launch_bounds__(64 * kW) void shared_attn_kernel(SharedParams a) {
     int page = p_first + w;
     const int code_end = min(p_end, code_pages);
     if (page < code_end) {
-        PageRaw<D, BITS> cur, nxt;
-        load(cur, page);
+        PageRaw<D, BITS> r;
+        load(r, page);
         while (true) {
-            const int np = page + kW;
-            const bool more = np < code_end;
-            load(nxt, more ? np : page);                 // unconditional: in flight while this page is computed
-            code_page(cur, page);
-            page = np;
-            if (!more) break;
-            cur = nxt;
+            code_page(r, page);
+            page += kW;
+            if (page >= code_end) break;
+            load(r, page);
         }
     }
     if (page < p_end) tail_page(page);                   // page == code_pages: only the partial one is left
@@ -935,56 +934,71 @@ void shared_tile_kernel(SharedParams a) {
     }
 }
 
-// Joins the shares of a row: prefix splits, then suffix splits, in order.  D/4 lanes a row,
-// four channels a lane.
+// Joins the shares of a row: prefix splits, then suffix splits.  D/4 lanes take four channels
+// each of every kMG-th share (its loads all go out before the first is used: the kernel is
+// little but the latency of reading the shares), and the kMG groups meet in LDS, in order.
+constexpr int kMG = 4;
 template <int D>
 __global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams a) {
-    constexpr int LPR = D / 4;
-    const int64_t idx = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / LPR;
-    const int ch = 4 * (threadIdx.x % LPR);
-    if (idx >= (int64_t)a.B * a.Hq * a.Sq) return;
+    constexpr int LPR = D / 4, RPB = kThreads / (LPR * kMG), NL = 8;
+    __shared__ v4f s_o[kMG - 1][RPB][LPR];
+    __shared__ float2 s_ml[kMG - 1][RPB];
+    const int ln = threadIdx.x % LPR, mg = threadIdx.x / LPR % kMG, rb = threadIdx.x / (LPR * kMG);
+    const int64_t rows = (int64_t)a.B * a.Hq * a.Sq;
+    const int64_t idx = min((int64_t)blockIdx.x * RPB + rb, rows - 1);
+    const bool on = (int64_t)blockIdx.x * RPB + rb < rows;
+    const int ch = 4 * ln;
     // rows as the prefix has them: ((kv head, b), i, g)
     const int g = (int)(idx % a.G), i = (int)(idx / a.G % a.Sq);
     const int b = (int)(idx / (a.G * a.Sq) % a.B), h = (int)(idx / ((int64_t)a.G * a.Sq * a.B));
+    const int n0 = a.p[0].splits, n = n0 + a.p[1].splits;
+    const int64_t all0 = (int64_t)a.Hkv * n0 * a.p[0].rows, all1 = (int64_t)a.p[1].items * a.Hkv * a.p[1].splits * a.p[1].rows;
+    const int64_t base0 = (int64_t)h * n0 * a.p[0].rows + (b * a.Sq + i) * a.G + g;
+    const int64_t base1 = (int64_t)(b * a.Hkv + h) * a.p[1].splits * a.p[1].rows + i * a.G + g;
     float M = -INFINITY, l = 0.f;
     v4f o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-        const SharedPart& P = a.p[p];
-        const int item = p == 1 ? b : 0;
-        const int row = p == 1 ? i * a.G + g : (b * a.Sq + i) * a.G + g;
-        const int64_t all = (int64_t)P.items * a.Hkv * P.splits * P.rows;
-        const int64_t base = (int64_t)(item * a.Hkv + h) * P.splits * P.rows + row;
-        for (int s0 = 0; s0 < P.splits; s0 += 4) {
-            float2 ml[4];
-            v4f x[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int64_t at = base + (int64_t)min(s0 + u, P.splits - 1) * P.rows;
-                ml[u] = *(const float2*)(P.part + all * D + 2 * at);
-                x[u] = *(const v4f*)(P.part + at * D + ch);
-            }
-            float mn = M;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) mn = fmaxf(mn, ml[u].x);
-            if (mn == -INFINITY) {       // nothing so far, but a NaN stays one
-#pragma unroll
-                for (int u = 0; u < 4; ++u) if (s0 + u < P.splits) { l += ml[u].y; o += x[u]; }
-                continue;
-            }
-            const float al = __builtin_amdgcn_exp2f(M - mn);
-            l *= al;
-            o *= al;
-            M = mn;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (s0 + u >= P.splits) break;
-                const float wt = __builtin_amdgcn_exp2f(ml[u].x - mn);
-                l = fmaf(wt, ml[u].y, l);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[r] = fmaf(wt, x[u][r], o[r]);
-            }
+    auto join = [&](float m, float pl, v4f x) __attribute__((always_inline)) {
+        const float mn = fmaxf(M, m);
+        if (mn == -INFINITY) {           // nothing so far, but a NaN stays one
+            l += pl;
+            o += x;
+            return;
         }
+        const float wa = __builtin_amdgcn_exp2f(M - mn), wb = __builtin_amdgcn_exp2f(m - mn);
+        M = mn;
+        l = fmaf(wb, pl, wa * l);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = fmaf(wb, x[r], wa * o[r]);
+    };
+    for (int s0 = mg; s0 < n; s0 += kMG * NL) {
+        float2 ml[NL];
+        v4f x[NL];
+#pragma unroll
+        for (int u = 0; u < NL; ++u) {
+            const int sp = s0 + kMG * u;
+            if (sp >= n) break;
+            const bool pre = sp < n0;
+            const float* part = pre ? a.p[0].part : a.p[1].part;
+            const int64_t at = pre ? base0 + (int64_t)sp * a.p[0].rows : base1 + (int64_t)(sp - n0) * a.p[1].rows;
+            ml[u] = *(const float2*)(part + (pre ? all0 : all1) * D + 2 * at);
+            x[u] = *(const v4f*)(part + at * D + ch);
+        }
+#pragma unroll
+        for (int u = 0; u < NL; ++u) {
+            if (s0 + kMG * u >= n) break;
+            join(ml[u].x, ml[u].y, x[u]);
+        }
+    }
+    if (mg > 0) {
+        s_o[mg - 1][rb][ln] = o;
+        if (ln == 0) s_ml[mg - 1][rb] = make_float2(M, l);
+    }
+    __syncthreads();
+    if (mg > 0 || !on) return;
+#pragma unroll
+    for (int u = 0; u < kMG - 1; ++u) {
+        const float2 ml = s_ml[u][rb];
+        join(ml.x, ml.y, s_o[u][rb][ln]);
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;         // a row without keys: O = 0, lse = -inf
     const int hq = h * a.G + g;
@@ -998,18 +1012,17 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams a) 
             l == 0.f ? -INFINITY : (M - kPShift + __log2f(l)) * kLn2;
 }
 
-// How a part's rows are taken: 16 or 32 rows a wave (nb 1, 2: shared_attn_kernel), or 256 / kg
-// rows a workgroup over stages in LDS (kg 1, 2, 4: shared_tile_kernel).
-struct Form { int nb, kg; };
+// How a part's rows are taken: 16 rows a wave (kg 0: shared_attn_kernel), or 256 / kg rows a
+// workgroup over stages in LDS (kg 1, 2, 4: shared_tile_kernel).
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Tiles and key splits of a part under a form: splits are chosen so that the workgroups fill
 // the GPU's slots once or a few times evenly.
-void plan_part(SharedPart& p, int Hkv, const Form& f) {
-    const bool tile = f.kg > 0;
+void plan_part(SharedPart& p, int Hkv, int kg) {
+    const bool tile = kg > 0;
     const int slots = tile ? 256 : 512;
-    const int rt = tile ? 256 / f.kg : 16 * f.nb;
+    const int rt = tile ? 256 / kg : 16;
     p.tiles = (int)ceil_div(p.rows, rt);
     p.pages = (int)ceil_div(p.keys, kPg);
     const int units = tile ? (int)ceil_div(p.pages, 2) : p.pages;
@@ -1022,10 +1035,7 @@ void plan_part(SharedPart& p, int Hkv, const Form& f) {
     p.wgs = groups * p.splits;
 }
 
-Form form_of(int rows) {
-    if (rows <= 16) return {1, 0};
-    return {2, rows <= 64 ? 4 : rows <= 128 ? 2 : 1};
-}
+int form_of(int rows) { return rows <= 16 ? 0 : rows <= 64 ? 4 : rows <= 128 ? 2 : 1; }
 
 size_t part_floats(const SharedPart& p, int Hkv, int D) {
     return (size_t)p.items * Hkv * p.splits * p.rows * (D + 2);
@@ -1041,10 +1051,10 @@ hipError_t launch_shared_prefix(const Int4Cache& pc, const TailArgs& pt, const I
     const int G = q.H_q / pc.Hkv;
     a.p[0].c = pc; a.p[0].t = pt; a.p[0].keys = pc.S + pt.len; a.p[0].items = 1; a.p[0].rows = q.B * q.S_q * G;
     a.p[1].c = sc; a.p[1].t = st_; a.p[1].keys = sc.S + st_.len; a.p[1].items = q.B; a.p[1].rows = q.S_q * G;
-    Form f[2];
+    int kg[2];
     for (int i = 0; i < 2; ++i) {
-        f[i] = form_of(a.p[i].rows);
-        plan_part(a.p[i], pc.Hkv, f[i]);
+        kg[i] = form_of(a.p[i].rows);
+        plan_part(a.p[i], pc.Hkv, kg[i]);
     }
     if (!ws) {
         *bytes = (part_floats(a.p[0], pc.Hkv, pc.D) + part_floats(a.p[1], pc.Hkv, pc.D)) * sizeof(float);
@@ -1058,25 +1068,25 @@ hipError_t launch_shared_prefix(const Int4Cache& pc, const TailArgs& pt, const I
     a.bf16 = q.dtype == FQ_BF16;
     a.B = q.B; a.Hq = q.H_q; a.Hkv = pc.Hkv; a.G = G; a.Sq = q.S_q;
     a.qk_scale = qk_scale;
-    auto attend = [&](int first, int last, const Form& f) {
+    auto attend = [&](int first, int last, int kg) {
         a.first = first; a.last = last;
         int64_t wgs = 0;
         for (int i = first; i <= last; ++i) wgs += a.p[i].wgs;
         const dim3 grid((unsigned)wgs);
         const bool bf = pc.meta_dtype == FQ_BF16;
-#define FQ_SP(D_, B_, Q_)                                                                                              \
-    if (pc.D == D_ && pc.bits == B_ && f.kg == 0 && f.nb == Q_) {                                                      \
-        if (bf) hipLaunchKernelGGL((shared_attn_kernel<D_, B_, bf16, Q_>), grid, dim3(64 * kW), 0, st, a);             \
-        else hipLaunchKernelGGL((shared_attn_kernel<D_, B_, f16, Q_>), grid, dim3(64 * kW), 0, st, a);                 \
+#define FQ_SP(D_, B_)                                                                                                  \
+    if (pc.D == D_ && pc.bits == B_ && kg == 0) {                                                                      \
+        if (bf) hipLaunchKernelGGL((shared_attn_kernel<D_, B_, bf16>), grid, dim3(64 * kW), 0, st, a);                 \
+        else hipLaunchKernelGGL((shared_attn_kernel<D_, B_, f16>), grid, dim3(64 * kW), 0, st, a);                     \
         return hipGetLastError();                                                                                      \
     }
 #define FQ_ST(D_, B_, K_)                                                                                              \
-    if (pc.D == D_ && pc.bits == B_ && f.kg == K_) {                                                                   \
+    if (pc.D == D_ && pc.bits == B_ && kg == K_) {                                                                     \
         if (bf) hipLaunchKernelGGL((shared_tile_kernel<D_, B_, bf16, K_>), grid, dim3(64 * kTW), 0, st, a);            \
         else hipLaunchKernelGGL((shared_tile_kernel<D_, B_, f16, K_>), grid, dim3(64 * kTW), 0, st, a);                \
         return hipGetLastError();                                                                                      \
     }
-#define FQ_SPQ(D_, B_) FQ_SP(D_, B_, 1) FQ_SP(D_, B_, 2) FQ_ST(D_, B_, 1) FQ_ST(D_, B_, 2) FQ_ST(D_, B_, 4)
+#define FQ_SPQ(D_, B_) FQ_SP(D_, B_) FQ_ST(D_, B_, 1) FQ_ST(D_, B_, 2) FQ_ST(D_, B_, 4)
         FQ_SPQ(128, 4) FQ_SPQ(128, 8) FQ_SPQ(64, 4) FQ_SPQ(64, 8)
 #undef FQ_SPQ
 #undef FQ_ST
@@ -1084,15 +1094,15 @@ hipError_t launch_shared_prefix(const Int4Cache& pc, const TailArgs& pt, const I
         return hipErrorInvalidValue;
     };
     hipError_t e;
-    if (f[0].kg == f[1].kg && (f[0].kg > 0 || f[0].nb == f[1].nb)) {
-        e = attend(0, 1, f[0]);
+    if (kg[0] == kg[1]) {
+        e = attend(0, 1, kg[0]);
     } else {
-        e = attend(0, 0, f[0]);
-        if (e == hipSuccess) e = attend(1, 1, f[1]);
+        e = attend(0, 0, kg[0]);
+        if (e == hipSuccess) e = attend(1, 1, kg[1]);
     }
     if (e != hipSuccess) return e;
-    const int64_t threads = (int64_t)q.B * q.H_q * q.S_q * (pc.D / 4);
-    const dim3 grid((unsigned)((threads + kThreads - 1) / kThreads));
+    const int64_t rows = (int64_t)q.B * q.H_q * q.S_q;
+    const dim3 grid((unsigned)ceil_div(rows, kThreads / (pc.D / 4 * kMG)));
     if (pc.D == 128) hipLaunchKernelGGL(shared_merge_kernel<128>, grid, dim3(kThreads), 0, st, a);
     else hipLaunchKernelGGL(shared_merge_kernel<64>, grid, dim3(kThreads), 0, st, a);
     return hipGetLastError();
