@@ -17,11 +17,19 @@
 // products: B S_q G rows against one set of keys, so a page that was loaded and turned into
 // operands serves all rows of a tile.  The suffix's rows are one sequence's S_q G.
 //
-// A wave takes 16 QB rows and every fourth page of its workgroup's range:
+// Both kernels compute the transposed products
 //   S^T = K Q^T     v_mfma_f32_16x16x32_f16, keys as the A operand
 //   O^T += V^T P^T  the same, channels as the A operand
-// The transposed products keep a row on one lane column: its statistics are per lane, and P
-// leaves S^T's accumulator as the B operand of the second product.
+// which keep a row on one lane column: its statistics are per lane, and P leaves S^T's
+// accumulator as the B operand of the second product.  shared_attn_kernel (few rows) turns the
+// codes into operands in registers, 16 rows a wave; shared_tile_kernel (many) once per workgroup
+// of 128 or 256 rows, through LDS.  plan_forms chooses, per part.
+//
+// What bounds them: reading the packed caches is the floor of short batches (37 MB of codes and
+// metadata for 32768 tokens of 8 KV heads in INT4: 7 us), the products that of long ones, and
+// between the two it is the vector instructions that turn codes into operands and scores into
+// weights: beyond two vector instructions a matrix instruction each further one adds its own
+// four cycles, so they have to be few of each page.
 //
 // Operands are fp16, whose 11 bits leave errors below those of 16-bit outputs (bf16's 8 do
 // not): q exact after a power of two per row (16-bit inputs), K and V one rounding of
@@ -56,7 +64,7 @@ struct SharedPart {
     int rows;                            // rows of an item and KV head
     int items, tiles, splits;            // sequences, row tiles, key splits
     int pages, per_split;                // pages (the partial one last), pages (row-tile kernel: stages) of a split
-    int64_t wgs;                         // items * Hkv * tiles * splits
+    uint32_t wgs;                        // items * Hkv * tiles * splits
     float* part;                         // [item][kv head][split][row]: D sums, then all (m, l)
 };
 
@@ -183,6 +191,22 @@ FQ_DEV uint32_t tail_pair(uint32_t wa, uint32_t wb, int odd) {
                : pack_h2(bf16_bits_to_f(wa & 0xFFFFu), bf16_bits_to_f(wb & 0xFFFFu));
 }
 
+// A workgroup's share: KV heads vary fastest, so with 8 of them the row tiles of a head and
+// range run on one XCD and share its L2.
+struct WgPlace { int h, tile, split, item; };
+FQ_DEV WgPlace place(const SharedPart& P, uint32_t blk, int Hkv) {
+    const uint32_t r1 = blk / Hkv, r2 = r1 / P.tiles;
+    return {(int)(blk - r1 * Hkv), (int)(r1 - r2 * P.tiles), (int)(r2 % P.splits), (int)(r2 / P.splits)};
+}
+
+// A row of a part: head in the group, token, sequence (item: the suffix's).
+struct RowPlace { int g, i, b; };
+FQ_DEV RowPlace row_place(uint32_t row, int G, int Sq, bool suffix, int item) {
+    const uint32_t t = row / G;
+    const uint32_t b = suffix ? 0 : t / Sq;
+    return {(int)(row - t * G), (int)(t - b * Sq), suffix ? item : (int)b};
+}
+
 // One step of the running softmax over a product's scores s (S^T: a lane's rows are its column's,
 // keys 16 T + 4 lg + r): p = 2^(s rs - reference + kPShift) as the B operands of the second
 // product.  The reference is the largest score seen, but moves only when one exceeds it by 2^8:
@@ -278,6 +302,11 @@ struct alignas(16) WaveMeta {
 // The keys of a lane's k-slots of step j of the second product: 32 j + 4 lg + {0..3}, then + 16.
 FQ_DEV constexpr int slot_key(int u) { return (u & 3) + 16 * (u >> 2); }      // u = 0 .. 7, before 32 j + 4 lg
 
+// Few rows: a wave takes 16 rows and every fourth page of its workgroup's range, its loads and
+// operands its own, and the four waves' states meet in LDS.  The loads of a page are not in
+// flight during the page before: with two waves a SIMD the other wave fills the wait, and the
+// registers for a second page would leave room for one (the suffixes of 64 sequences, INT8: 24 us
+// then, 14 now; three or four waves a SIMD spill and are slower).
 template <int D, int BITS, typename MT>
 __global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void shared_attn_kernel(SharedParams a) {
@@ -291,17 +320,10 @@ void shared_attn_kernel(SharedParams a) {
     const int n = L & 15, lg = L >> 4;
     WaveMeta<D>& M = s_meta[w];
 
-    // KV heads vary fastest over the workgroups, so with 8 of them the row tiles of a head and
-    // range run on one XCD and share its L2
-    int64_t blk = blockIdx.x;
-    const int pi = a.first < a.last && blk >= a.p[0].wgs ? 1 : a.first;
-    if (pi > a.first) blk -= a.p[0].wgs;
+    const int pi = a.first < a.last && blockIdx.x >= a.p[0].wgs ? 1 : a.first;
     const SharedPart& P = a.p[pi];
-    const int h = (int)(blk % a.Hkv);
-    const int64_t r1 = blk / a.Hkv;
-    const int tile = (int)(r1 % P.tiles);
-    const int64_t r2 = r1 / P.tiles;
-    const int split = (int)(r2 % P.splits), item = (int)(r2 / P.splits);
+    const WgPlace at = place(P, blockIdx.x - (pi > a.first ? a.p[0].wgs : 0u), a.Hkv);
+    const int h = at.h, tile = at.tile, split = at.split, item = at.item;
     const Int4Cache& c = P.c;
     const int code_pages = c.S / kPg;
 
@@ -318,9 +340,9 @@ void shared_attn_kernel(SharedParams a) {
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
         const int row = min(row0 + 16 * qb + n, P.rows - 1);
-        const int g = row % a.G, i = (row / a.G) % a.Sq, b = pi == 1 ? item : row / (a.G * a.Sq);
-        hi[qb] = pi == 1 ? P.keys - a.Sq + i : P.keys - 1;
-        const uint16_t* q = (const uint16_t*)a.q + b * a.q_s[0] + (int64_t)(h * a.G + g) * a.q_s[1] + i * a.q_s[2];
+        const RowPlace r = row_place(row, a.G, a.Sq, pi == 1, item);
+        hi[qb] = pi == 1 ? P.keys - a.Sq + r.i : P.keys - 1;
+        const uint16_t* q = (const uint16_t*)a.q + r.b * a.q_s[0] + (int64_t)(h * a.G + r.g) * a.q_s[1] + r.i * a.q_s[2];
         rs[qb] = load_query<D, BITS>(q, (D / 4) * lg, 8, a.bf16, a.qk_scale, qf[qb]);
     }
 
@@ -620,7 +642,7 @@ void shared_tile_kernel(SharedParams a) {
     constexpr int QB = 2, NS = D / 32, NT = D / 16, VC = D / 16;
     constexpr int RG = kTW / KG;                 // row groups
     constexpr int RT = 32 * RG;                  // rows of the workgroup
-    constexpr int SUB = KG == 4 ? 32 : 64;       // keys of a wave's product
+    constexpr int SUB = 64;                      // keys of a wave's product
     constexpr int NK = SUB / 16, NJ = SUB / 32, NSUB = kST / KG / SUB;       // 16-key tiles, 32-key steps, products a stage
     constexpr int CPR = D / 8, KPT = D / 32;     // K: chunks of a row, rows a thread turns
     constexpr int KW = BITS / 4, VW = VC * BITS / 8 == 8 ? 2 : 1;            // dwords of 8 K channels, of VC V channels
@@ -631,15 +653,10 @@ void shared_tile_kernel(SharedParams a) {
     const int tid = threadIdx.x, L = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_id());
     const int n = L & 15, lg = L >> 4;
 
-    int64_t blk = blockIdx.x;
-    const int pi = a.first < a.last && blk >= a.p[0].wgs ? 1 : a.first;
-    if (pi > a.first) blk -= a.p[0].wgs;
+    const int pi = a.first < a.last && blockIdx.x >= a.p[0].wgs ? 1 : a.first;
     const SharedPart& P = a.p[pi];
-    const int h = (int)(blk % a.Hkv);
-    const int64_t r1 = blk / a.Hkv;
-    const int tile = (int)(r1 % P.tiles);
-    const int64_t r2 = r1 / P.tiles;
-    const int split = (int)(r2 % P.splits), item = (int)(r2 / P.splits);
+    const WgPlace at = place(P, blockIdx.x - (pi > a.first ? a.p[0].wgs : 0u), a.Hkv);
+    const int h = at.h, tile = at.tile, split = at.split, item = at.item;
     const Int4Cache& c = P.c;
     const int code_pages = c.S / kPg;
     const int kg = w / RG;                       // key group
@@ -656,9 +673,9 @@ void shared_tile_kernel(SharedParams a) {
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
         const int row = min(row0 + 16 * qb + n, P.rows - 1);
-        const int g = row % a.G, i = (row / a.G) % a.Sq, b = pi == 1 ? item : row / (a.G * a.Sq);
-        hi[qb] = pi == 1 ? P.keys - a.Sq + i : P.keys - 1;
-        const uint16_t* q = (const uint16_t*)a.q + b * a.q_s[0] + (int64_t)(h * a.G + g) * a.q_s[1] + i * a.q_s[2];
+        const RowPlace r = row_place(row, a.G, a.Sq, pi == 1, item);
+        hi[qb] = pi == 1 ? P.keys - a.Sq + r.i : P.keys - 1;
+        const uint16_t* q = (const uint16_t*)a.q + r.b * a.q_s[0] + (int64_t)(h * a.G + r.g) * a.q_s[1] + r.i * a.q_s[2];
         rs[qb] = load_query<D, BITS>(q, 8 * lg, 32, a.bf16, a.qk_scale, qf[qb]);
     }
 
@@ -935,25 +952,24 @@ void shared_tile_kernel(SharedParams a) {
 }
 
 // Joins the shares of a row: prefix splits, then suffix splits.  D/4 lanes take four channels
-// each of every kMG-th share (its loads all go out before the first is used: the kernel is
-// little but the latency of reading the shares), and the kMG groups meet in LDS, in order.
-constexpr int kMG = 4;
-template <int D>
+// each of every MG-th share (its loads all go out before the first is used: the kernel is
+// little but the latency of reading the shares), and the MG groups meet in LDS, in order.
+template <int D, int MG>
 __global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams a) {
-    constexpr int LPR = D / 4, RPB = kThreads / (LPR * kMG), NL = 8;
-    __shared__ v4f s_o[kMG - 1][RPB][LPR];
-    __shared__ float2 s_ml[kMG - 1][RPB];
-    const int ln = threadIdx.x % LPR, mg = threadIdx.x / LPR % kMG, rb = threadIdx.x / (LPR * kMG);
-    const int64_t rows = (int64_t)a.B * a.Hq * a.Sq;
-    const int64_t idx = min((int64_t)blockIdx.x * RPB + rb, rows - 1);
-    const bool on = (int64_t)blockIdx.x * RPB + rb < rows;
+    constexpr int LPR = D / 4, RPB = kThreads / (LPR * MG), NL = 8;
+    __shared__ v4f s_o[MG][RPB][LPR];            // (group 0's stays in its registers)
+    __shared__ float2 s_ml[MG][RPB];
+    const int ln = threadIdx.x % LPR, mg = threadIdx.x / LPR % MG, rb = threadIdx.x / (LPR * MG);
+    const uint32_t rows = a.B * a.Hq * a.Sq, at = blockIdx.x * RPB + rb;
+    const bool on = at < rows;
     const int ch = 4 * ln;
     // rows as the prefix has them: ((kv head, b), i, g)
-    const int g = (int)(idx % a.G), i = (int)(idx / a.G % a.Sq);
-    const int b = (int)(idx / (a.G * a.Sq) % a.B), h = (int)(idx / ((int64_t)a.G * a.Sq * a.B));
+    const uint32_t idx = min(at, rows - 1), h = idx / a.p[0].rows, prow = idx - h * a.p[0].rows;
+    const RowPlace rp = row_place(prow, a.G, a.Sq, false, 0);
+    const int g = rp.g, i = rp.i, b = rp.b;
     const int n0 = a.p[0].splits, n = n0 + a.p[1].splits;
     const int64_t all0 = (int64_t)a.Hkv * n0 * a.p[0].rows, all1 = (int64_t)a.p[1].items * a.Hkv * a.p[1].splits * a.p[1].rows;
-    const int64_t base0 = (int64_t)h * n0 * a.p[0].rows + (b * a.Sq + i) * a.G + g;
+    const int64_t base0 = (int64_t)h * n0 * a.p[0].rows + prow;
     const int64_t base1 = (int64_t)(b * a.Hkv + h) * a.p[1].splits * a.p[1].rows + i * a.G + g;
     float M = -INFINITY, l = 0.f;
     v4f o = {0.f, 0.f, 0.f, 0.f};
@@ -970,12 +986,12 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams a) 
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] = fmaf(wb, x[r], wa * o[r]);
     };
-    for (int s0 = mg; s0 < n; s0 += kMG * NL) {
+    for (int s0 = mg; s0 < n; s0 += MG * NL) {
         float2 ml[NL];
         v4f x[NL];
 #pragma unroll
         for (int u = 0; u < NL; ++u) {
-            const int sp = s0 + kMG * u;
+            const int sp = s0 + MG * u;
             if (sp >= n) break;
             const bool pre = sp < n0;
             const float* part = pre ? a.p[0].part : a.p[1].part;
@@ -985,18 +1001,20 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams a) 
         }
 #pragma unroll
         for (int u = 0; u < NL; ++u) {
-            if (s0 + kMG * u >= n) break;
+            if (s0 + MG * u >= n) break;
             join(ml[u].x, ml[u].y, x[u]);
         }
     }
-    if (mg > 0) {
-        s_o[mg - 1][rb][ln] = o;
-        if (ln == 0) s_ml[mg - 1][rb] = make_float2(M, l);
+    if constexpr (MG > 1) {
+        if (mg > 0) {
+            s_o[mg][rb][ln] = o;
+            if (ln == 0) s_ml[mg][rb] = make_float2(M, l);
+        }
+        __syncthreads();
     }
-    __syncthreads();
     if (mg > 0 || !on) return;
 #pragma unroll
-    for (int u = 0; u < kMG - 1; ++u) {
+    for (int u = 1; u < MG; ++u) {
         const float2 ml = s_ml[u][rb];
         join(ml.x, ml.y, s_o[u][rb][ln]);
     }
@@ -1013,29 +1031,62 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(SharedParams a) 
 }
 
 // How a part's rows are taken: 16 rows a wave (kg 0: shared_attn_kernel), or 256 / kg rows a
-// workgroup over stages in LDS (kg 1, 2, 4: shared_tile_kernel).
-
+// workgroup over stages in LDS (kg 1, 2: shared_tile_kernel).
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Tiles and key splits of a part under a form: splits are chosen so that the workgroups fill
-// the GPU's slots once or a few times evenly.
-void plan_part(SharedPart& p, int Hkv, int kg) {
-    const bool tile = kg > 0;
-    const int slots = tile ? 256 : 512;
-    const int rt = tile ? 256 / kg : 16;
+// A part under a form; `pages_a_wg`: what a workgroup of 16-row waves should take.
+void plan_part(SharedPart& p, int Hkv, int kg, int64_t pages_a_wg) {
+    const int rt = kg ? 256 / kg : 16;
     p.tiles = (int)ceil_div(p.rows, rt);
     p.pages = (int)ceil_div(p.keys, kPg);
-    const int units = tile ? (int)ceil_div(p.pages, 2) : p.pages;
     const int64_t groups = (int64_t)p.items * Hkv * p.tiles;
-    const int most = std::max<int>(1, (int)(tile ? ceil_div(units, 2) : ceil_div(units, kW)));
-    int64_t s = std::max<int64_t>(1, slots / std::max<int64_t>(1, groups));
-    s = std::min<int64_t>(s, most);
-    p.per_split = std::max(1, (int)ceil_div(units, s));
-    p.splits = std::max(1, (int)ceil_div(units, p.per_split));
-    p.wgs = groups * p.splits;
+    if (kg) {       // one workgroup a CU; at least two stages each
+        const int stages = (int)ceil_div(p.pages, 2);
+        const int64_t s = std::min(std::max<int64_t>(1, 256 / groups), ceil_div(stages, 2));
+        p.per_split = (int)ceil_div(stages, s);
+        p.splits = (int)ceil_div(stages, p.per_split);
+    } else {
+        p.per_split = (int)std::min<int64_t>(p.pages, pages_a_wg);
+        p.splits = (int)ceil_div(p.pages, p.per_split);
+    }
+    p.wgs = (uint32_t)(groups * p.splits);
 }
 
-int form_of(int rows) { return rows <= 16 ? 0 : rows <= 64 ? 4 : rows <= 128 ? 2 : 1; }
+// Forms of the two parts and their plans: the least time by a model fitted to 24 .. 1024 rows
+// over 512 .. 32768 tokens (us; D = 128, INT4 / INT8 in the same words, D = 64 below):
+//   16-row waves   1.4e-3 / 1.6e-3 a page of a wave, 10 a step in all where both parts go this way
+//   row tiles      4.6 / 2.7 a stage of 256 / 128 rows on every CU, and 12 / 10 a launch for its
+//                  start, the first stage and the shares
+// 64 rows over 32768 tokens: 36 us with waves, 42 with tiles; 128 rows: 57 and 48; 512 rows over
+// 2048: 33 and 43, over 32768: 192 and 102 (tiles of 256 rows; 109 of 128).
+void plan_forms(SharedParams& a, int D, int bits, int (&kg)[2]) {
+    const double wave = D == 128 ? (bits == 4 ? 1.4e-3 : 1.6e-3) : 0.9e-3;
+    const double stage[3] = {0., D == 128 ? 4.6 : 3.2, D == 128 ? 2.7 : 2.0}, start[3] = {0., 12., 10.};
+    constexpr int kSlots = 512;         // workgroups of 16-row waves that run at once
+    double best = 0.;
+    SharedPart plan[2];
+    for (int k0 = 0; k0 < 3; ++k0)
+        for (int k1 = 0; k1 < 3; ++k1) {
+            SharedPart p[2] = {a.p[0], a.p[1]};
+            const int k[2] = {k0, k1};
+            double pages = 0., t = k0 == k1 ? 0. : 5.;      // pages of 16-row waves; another launch
+            for (int i = 0; i < 2; ++i)
+                if (!k[i]) pages += (double)p[i].items * a.Hkv * ceil_div(p[i].rows, 16) * ceil_div(p[i].keys, kPg);
+            const int64_t each = std::max<int64_t>(kW, ceil_div((int64_t)pages, kSlots));
+            for (int i = 0; i < 2; ++i) {
+                plan_part(p[i], a.Hkv, k[i], each);
+                if (k[i]) t += (i == 1 && k0 == k1 ? 0. : start[k[i]]) + (double)ceil_div(p[i].wgs, 256) * p[i].per_split * stage[k[i]];
+            }
+            t += pages * wave;
+            if (best == 0. || t < best) {
+                best = t;
+                kg[0] = k0; kg[1] = k1;
+                plan[0] = p[0]; plan[1] = p[1];
+            }
+        }
+    a.p[0] = plan[0];
+    a.p[1] = plan[1];
+}
 
 size_t part_floats(const SharedPart& p, int Hkv, int D) {
     return (size_t)p.items * Hkv * p.splits * p.rows * (D + 2);
@@ -1051,28 +1102,23 @@ hipError_t launch_shared_prefix(const Int4Cache& pc, const TailArgs& pt, const I
     const int G = q.H_q / pc.Hkv;
     a.p[0].c = pc; a.p[0].t = pt; a.p[0].keys = pc.S + pt.len; a.p[0].items = 1; a.p[0].rows = q.B * q.S_q * G;
     a.p[1].c = sc; a.p[1].t = st_; a.p[1].keys = sc.S + st_.len; a.p[1].items = q.B; a.p[1].rows = q.S_q * G;
+    a.Hkv = pc.Hkv;
     int kg[2];
-    for (int i = 0; i < 2; ++i) {
-        kg[i] = form_of(a.p[i].rows);
-        plan_part(a.p[i], pc.Hkv, kg[i]);
-    }
+    plan_forms(a, pc.D, pc.bits, kg);
     if (!ws) {
         *bytes = (part_floats(a.p[0], pc.Hkv, pc.D) + part_floats(a.p[1], pc.Hkv, pc.D)) * sizeof(float);
         return hipSuccess;
     }
-    if (a.p[0].wgs + a.p[1].wgs > 0x7FFFFFFF) return hipErrorInvalidValue;
     a.p[0].part = (float*)ws;
     a.p[1].part = a.p[0].part + part_floats(a.p[0], pc.Hkv, pc.D);
     a.q = q.q; a.out = q.out; a.lse = q.lse; a.start = q.start;
     for (int i = 0; i < 3; ++i) { a.q_s[i] = q.q_strides[i]; a.o_s[i] = q.o_strides[i]; a.lse_s[i] = q.lse_strides[i]; }
     a.bf16 = q.dtype == FQ_BF16;
-    a.B = q.B; a.Hq = q.H_q; a.Hkv = pc.Hkv; a.G = G; a.Sq = q.S_q;
+    a.B = q.B; a.Hq = q.H_q; a.G = G; a.Sq = q.S_q;
     a.qk_scale = qk_scale;
     auto attend = [&](int first, int last, int kg) {
         a.first = first; a.last = last;
-        int64_t wgs = 0;
-        for (int i = first; i <= last; ++i) wgs += a.p[i].wgs;
-        const dim3 grid((unsigned)wgs);
+        const dim3 grid((first == 0 ? a.p[0].wgs : 0) + (last == 1 ? a.p[1].wgs : 0));
         const bool bf = pc.meta_dtype == FQ_BF16;
 #define FQ_SP(D_, B_)                                                                                                  \
     if (pc.D == D_ && pc.bits == B_ && kg == 0) {                                                                      \
@@ -1086,7 +1132,7 @@ hipError_t launch_shared_prefix(const Int4Cache& pc, const TailArgs& pt, const I
         else hipLaunchKernelGGL((shared_tile_kernel<D_, B_, f16, K_>), grid, dim3(64 * kTW), 0, st, a);                \
         return hipGetLastError();                                                                                      \
     }
-#define FQ_SPQ(D_, B_) FQ_SP(D_, B_) FQ_ST(D_, B_, 1) FQ_ST(D_, B_, 2) FQ_ST(D_, B_, 4)
+#define FQ_SPQ(D_, B_) FQ_SP(D_, B_) FQ_ST(D_, B_, 1) FQ_ST(D_, B_, 2)
         FQ_SPQ(128, 4) FQ_SPQ(128, 8) FQ_SPQ(64, 4) FQ_SPQ(64, 8)
 #undef FQ_SPQ
 #undef FQ_ST
@@ -1102,9 +1148,13 @@ hipError_t launch_shared_prefix(const Int4Cache& pc, const TailArgs& pt, const I
     }
     if (e != hipSuccess) return e;
     const int64_t rows = (int64_t)q.B * q.H_q * q.S_q;
-    const dim3 grid((unsigned)ceil_div(rows, kThreads / (pc.D / 4 * kMG)));
-    if (pc.D == 128) hipLaunchKernelGGL(shared_merge_kernel<128>, grid, dim3(kThreads), 0, st, a);
-    else hipLaunchKernelGGL(shared_merge_kernel<64>, grid, dim3(kThreads), 0, st, a);
+    // four groups of lanes a row where there are shares for them
+    const int mg = a.p[0].splits + a.p[1].splits > 8 ? 4 : 1;
+    const dim3 grid((unsigned)ceil_div(rows, kThreads / (pc.D / 4 * mg)));
+    if (pc.D == 128 && mg == 4) hipLaunchKernelGGL((shared_merge_kernel<128, 4>), grid, dim3(kThreads), 0, st, a);
+    else if (pc.D == 128) hipLaunchKernelGGL((shared_merge_kernel<128, 1>), grid, dim3(kThreads), 0, st, a);
+    else if (mg == 4) hipLaunchKernelGGL((shared_merge_kernel<64, 4>), grid, dim3(kThreads), 0, st, a);
+    else hipLaunchKernelGGL((shared_merge_kernel<64, 1>), grid, dim3(kThreads), 0, st, a);
     return hipGetLastError();
 }
 
