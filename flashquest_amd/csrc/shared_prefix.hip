@@ -233,13 +233,13 @@ FQ_DEV void softmax_step(v4f (&s)[QB][NK], const float (&rs)[QB], float (&m_run)
             m = fmaxf(fmaxf(m, s[qb][T][0]), s[qb][T][1]);
             m = fmaxf(fmaxf(m, s[qb][T][2]), s[qb][T][3]);
         }
-        mx[qb] = rows_max(m);
-        moved |= mx[qb] > (none ? -INFINITY : kPShift + kLazy);
+        mx[qb] = m;                              // of this lane's keys: joined over the row's lanes if it matters
+        moved |= m > (none ? -INFINITY : kPShift + kLazy);
     }
     if (__builtin_amdgcn_ballot_w64(moved)) {
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
-            const float m_new = fmaxf(m_run[qb], mx[qb] - ref[qb]);
+            const float m_new = fmaxf(m_run[qb], rows_max(mx[qb]) - ref[qb]);
             const float nref = kPShift - (m_new == -INFINITY ? 0.f : m_new);
             const float al = __builtin_amdgcn_exp2f(m_run[qb] + nref - kPShift), by = nref - ref[qb];
             m_run[qb] = m_new;
@@ -598,13 +598,19 @@ void shared_attn_kernel(SharedParams a) {
 }
 
 // ---- many rows: keys and values staged in LDS ------------------------------------------
-// With more rows than a wave or two take, turning a page into operands once per 32 rows is
-// what the time goes into.  Here a workgroup of 8 waves turns each stage of 128 keys (two
-// pages) into fp16 once, K as [key][channel] and V as [channel][key] in LDS, while the stage
-// before is attended: 256 / KG rows (32 a wave) times KG groups of keys, key group kg taking
-// keys 128 kg / KG .. of every stage for its rows; the groups' states meet in LDS at the end.
-// The codes of stage t + 2 are loaded before stage t + 1 is written: no wait on memory in
-// the loop but the one for loads that are a stage old.
+// With more rows than a wave or two take, turning a page into operands once per 16 rows is what
+// the time goes into.  Here a workgroup turns each stage of two pages into fp16 once, K as
+// [key][channel] and V as [channel][key] in LDS, while the stage before is attended: 256 / KG rows
+// times KG groups of keys, key group kg taking keys 128 kg / KG .. of every stage for its rows; the
+// groups' states meet in LDS at the end.  Metadata is turned into fp16 once, through LDS too.  The
+// codes are loaded a stage ahead, their metadata two: no wait on memory in the loop but the one for
+// loads that are a stage old.
+//
+// KG = 1: 8 waves of 32 rows, two a SIMD, each thread turning K and V; an operand read from LDS
+// feeds two matrix instructions.  KG = 2: 16 waves of 16 rows, four a SIMD, the lower ones turning K
+// and the upper ones V; a read feeds one (1.9 ns of LDS to 1.8 of the four matrix cores), but three
+// other waves have work while one waits.  512 rows over 32768 tokens in INT4: 102 us with 8 waves for
+// KG = 1, 106 with 16; 128 rows: 49 with 8 for KG = 2, 47 with 16; 320 rows over 16384: 60 and 49.
 //
 // LDS holds a plane for each lane group lg of the operands: K's plane has a row per key of the
 // chunks (8 channels, 16 bytes) 4 st + lg, V's a row per channel of the chunks (8 keys) 4 jb + lg.
@@ -613,8 +619,7 @@ void shared_attn_kernel(SharedParams a) {
 // do the writes (planes 64 bytes apart modulo 256; not for K with D = 64, 4 on a bank).  V's
 // channels are dealt to the tiles as the codes unpack (tile i: channels D/16 n + i), so that the
 // 16 lanes that write channel i of their codes write neighbouring rows.
-constexpr int kTW = 8;                   // waves
-constexpr int kST = 128;                 // keys of a stage
+constexpr int kST = 2 * kPg;             // keys of a stage
 // Scheduling groups: n LDS reads, then (m matrix instructions, one read) until the reads are out,
 // then the rest: operand reads stay n ahead of their use (left alone, the scheduler puts each
 // right before it and every pair of matrix instructions waits for LDS).
@@ -628,6 +633,8 @@ FQ_DEV void reads_ahead() {
     }
     __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * MFMA_PER_READ, 0);
 }
+constexpr int tile_waves(int kg) { return kg == 1 ? 8 : 16; }
+
 template <int D> struct StageLds {
     static constexpr int NS = D / 32;
     static constexpr int KROW = 16 * NS, KPL = kST * KROW + (D == 128 ? 64 : 0), KB = 4 * KPL;
@@ -637,19 +644,22 @@ template <int D> struct StageLds {
 };
 
 template <int D, int BITS, typename MT, int KG>
-__global__ __launch_bounds__(64 * kTW) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(64 * tile_waves(KG)) __attribute__((amdgpu_waves_per_eu(tile_waves(KG) / 4, tile_waves(KG) / 4)))
 void shared_tile_kernel(SharedParams a) {
-    constexpr int QB = 2, NS = D / 32, NT = D / 16, VC = D / 16;
+    constexpr int kTW = tile_waves(KG), QB = 16 / kTW, NS = D / 32, NT = D / 16, VC = D / 16;
     constexpr int RG = kTW / KG;                 // row groups
-    constexpr int RT = 32 * RG;                  // rows of the workgroup
-    constexpr int SUB = 64;                      // keys of a wave's product
-    constexpr int NK = SUB / 16, NJ = SUB / 32, NSUB = kST / KG / SUB;       // 16-key tiles, 32-key steps, products a stage
-    constexpr int CPR = D / 8, KPT = D / 32;     // K: chunks of a row, rows a thread turns
+    constexpr int RT = 16 * QB * RG;                  // rows of the workgroup
+    constexpr int NK = kPg / 16, NJ = kPg / 32, NSUB = 2 / KG;       // of a product of 64 keys: 16-key tiles, 32-key steps; products a stage
+    constexpr int TPP = 256;                     // threads of a page (KG = 2: for K and for V)
+    constexpr int CPR = D / 8, KPT = kPg * CPR / TPP;        // K: chunks of a row, rows a thread turns
     constexpr int KW = BITS / 4, VW = VC * BITS / 8 == 8 ? 2 : 1;            // dwords of 8 K channels, of VC V channels
-    constexpr int AHEAD = 6;                     // operand reads in flight
+    constexpr int AHEAD = QB == 2 ? 6 : 2;                    // operand reads in flight
     using Lds = StageLds<D>;
     __shared__ __attribute__((aligned(16))) uint8_t s_k[2][Lds::KB];
     __shared__ __attribute__((aligned(16))) uint8_t s_v[2][Lds::VB];
+    // metadata as fp16, scales with the codes' factor: [stage & 1][page] [scale, minimum] of K's
+    // channels in operand order, and of V's tokens by channel group
+    __shared__ __attribute__((aligned(16))) uint16_t s_km[2][2][2][D], s_vm[2][2][4][2][kPg];
     const int tid = threadIdx.x, L = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_id());
     const int n = L & 15, lg = L >> 4;
 
@@ -660,7 +670,8 @@ void shared_tile_kernel(SharedParams a) {
     const Int4Cache& c = P.c;
     const int code_pages = c.S / kPg;
     const int kg = w / RG;                       // key group
-    const int wg_row0 = tile * RT, row0 = wg_row0 + (w % RG) * 32;
+    const int wg_row0 = tile * RT, row0 = wg_row0 + (w % RG) * (16 * QB);
+
     const bool wave_on = row0 < P.rows;
 
     int hi[QB], lo = 0, hi_all = P.keys - 1;
@@ -690,118 +701,129 @@ void shared_tile_kernel(SharedParams a) {
     }
     const v8h ones = frag(0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u);
 
-    // This thread's part of a stage: KPT keys' 8 channels of K and 4 keys' VC channels of V, of
-    // page 2 t + pg (a wave's threads are in one page).
-    const int pg = w >> 2;
-    const int kc = tid % CPR, kr = (tid & 255) / CPR;              // K: chunk, first row in the page
-    // V: channels VC vc .., keys 4 vq .. in the page (a wave's four vq fill whole 16-byte chunks)
-    const int vt = (tid >> 4) & 15, vc = tid & 15, vq = (vt & 8) | (vt & 1) << 2 | ((vt >> 1) & 3);
+    // This thread's part of a stage, of its page 2 t + pg: KPT keys' 8 channels of K, or 4 keys' VC
+    // channels of V, or both.
+    const bool upper = w >= kTW / 2;
+    constexpr auto takes_k = [](auto up) { return KG == 1 || !decltype(up)::value; };
+    constexpr auto takes_v = [](auto up) { return KG == 1 || decltype(up)::value; };
+    const int ti = tid & (TPP - 1), pg = (w >> 2) & 1;
+    const int kc = ti % CPR, kr = ti / CPR;      // K: chunk, first key
+    const int vc = ti & 15, vt = ti >> 4;        // V: channels VC vc .., keys 4 vq .. (a wave's four vq fill whole 16-byte chunks)
+    const int vq = (vt & 8) | (vt & 1) << 2 | ((vt >> 1) & 3);
     const uint8_t* kb = c.kp + item * c.kp_s[1] + h * c.kp_s[2] + kr * c.kp_s[3] + kc * BITS;
-    const uint8_t* vb = c.vp + item * c.vp_s[1] + h * c.vp_s[2] + 4 * vq * c.vp_s[3] + vc * (VC * BITS / 8);
-    const uint16_t* ksb = (const uint16_t*)c.ksc + item * c.ksc_s[1] + h * c.ksc_s[2] + 8 * kc;
-    const uint16_t* kmb = (const uint16_t*)c.kmn + item * c.kmn_s[1] + h * c.kmn_s[2] + 8 * kc;
+    const uint8_t* vb = c.vp + item * c.vp_s[1] + h * c.vp_s[2] + vc * (VC * BITS / 8) + 4 * vq * c.vp_s[3];
+    struct Raw { uint32_t k[KPT * KW], v[4 * VW]; };
+    // and of its metadata: K's scale or minimum of one channel, V's of one token in groups mg, mg + 2
+    const int mt = ti & 63, mg = __builtin_amdgcn_readfirstlane(ti >> 7);
+    const bool mv = ti & 64;
+    const uint16_t* vmeta = mv ? (const uint16_t*)c.vmn + item * c.vmn_s[1] + h * c.vmn_s[2] + mt * c.vmn_s[3] + mg
+                               : (const uint16_t*)c.vsc + item * c.vsc_s[1] + h * c.vsc_s[2] + mt * c.vsc_s[3] + mg;
+    const int64_t vmeta_s = kPg * (mv ? c.vmn_s[3] : c.vsc_s[3]);
+    const float vmeta_f = mv ? 1.f : kCodeUp<BITS>;
+    auto slot = [](int ch) { return BITS == 4 ? (ch & ~7) | (ch & 3) << 1 | ((ch >> 2) & 1) : ch; };      // operand order
     const int vg = vc * c.G >> 4;
-    const uint16_t* vsb = (const uint16_t*)c.vsc + item * c.vsc_s[1] + h * c.vsc_s[2] + 4 * vq * c.vsc_s[3] + vg;
-    const uint16_t* vmb = (const uint16_t*)c.vmn + item * c.vmn_s[1] + h * c.vmn_s[2] + 4 * vq * c.vmn_s[3] + vg;
-    struct Raw {
-        uint32_t k[KPT][KW], v[4][VW];
-        u32x4 ks, km;
-        uint32_t vs[4], vm[4];
-    };
-    auto load = [&](Raw& r, int t) __attribute__((always_inline)) {             // code pages; others are read when they are written
-        const int page = min(2 * t + pg, code_pages - 1);
-        if (page < 0) return;
-        const int64_t t0 = (int64_t)page * kPg;
+    struct RawMeta { uint32_t k, v[2]; };
+    const uint16_t* ksb = (const uint16_t*)c.ksc + item * c.ksc_s[1] + h * c.ksc_s[2] + (ti & (D - 1));
+    const uint16_t* kmb = (const uint16_t*)c.kmn + item * c.kmn_s[1] + h * c.kmn_s[2] + (ti & (D - 1));
+    const uint16_t* kmeta = ti & D ? kmb : ksb;
+    const int64_t kmeta_s = ti & D ? c.kmn_s[3] : c.ksc_s[3];
+    const int last_page = max(code_pages - 1, 0);        // later pages are not loaded ahead; S = 0: the host's dummies are read
+    auto load_meta = [&](auto up, RawMeta& r, int t) __attribute__((always_inline)) {
+        const int page = min(2 * t + pg, last_page);
+        if constexpr (takes_v(up)) {
+            const uint16_t* v = vmeta + page * vmeta_s;
 #pragma unroll
-        for (int j = 0; j < KPT; ++j) {
-            const uint8_t* p = kb + (t0 + 256 / CPR * j) * c.kp_s[3];
-            if constexpr (KW == 1) r.k[j][0] = *(const uint32_t*)p;
-            else { const u32x2 x = *(const u32x2*)p; r.k[j][0] = x.x; r.k[j][1] = x.y; }
+            for (int u = 0; u < 2; ++u)
+                if (mg + 2 * u < c.G) r.v[u] = v[2 * u];
         }
-        r.ks = *(const u32x4*)(ksb + page * c.ksc_s[3]);
-        r.km = *(const u32x4*)(kmb + page * c.kmn_s[3]);
+        if constexpr (takes_k(up)) r.k = kmeta[page * kmeta_s];
+    };
+    auto put_meta = [&](auto up, const RawMeta& r, int t) __attribute__((always_inline)) {
+        if constexpr (takes_v(up)) {
+            const bool on = (2 * t + pg) * kPg + mt >= lo;      // values of padding tokens count as 0, whatever they are
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint8_t* p = vb + (t0 + j) * c.vp_s[3];
-            if constexpr (VC * BITS == 16) r.v[j][0] = *(const uint16_t*)p;
-            else if constexpr (VW == 1) r.v[j][0] = *(const uint32_t*)p;
-            else { const u32x2 x = *(const u32x2*)p; r.v[j][0] = x.x; r.v[j][1] = x.y; }
-            r.vs[j] = vsb[(t0 + j) * c.vsc_s[3]];
-            r.vm[j] = vmb[(t0 + j) * c.vmn_s[3]];
+            for (int u = 0; u < 2; ++u)
+                if (mg + 2 * u < c.G) s_vm[t & 1][pg][mg + 2 * u][mv][mt] = on ? f_to_f16_bits(meta_f<MT>(r.v[u]) * vmeta_f) : 0;
+        }
+        if constexpr (takes_k(up)) {
+            const bool mn = ti & D;
+            if (ti < 2 * D) s_km[t & 1][pg][mn][slot(ti & (D - 1))] = f_to_f16_bits(meta_f<MT>(r.k) * (mn ? kKExp : kCodeUp<BITS> * kKExp));
+        }
+    };
+    auto load = [&](auto up, Raw& r, int t) __attribute__((always_inline)) {    // code pages; the partial one is read when it is written
+        const int64_t t0 = (int64_t)min(2 * t + pg, last_page) * kPg;
+        if constexpr (takes_k(up)) {
+#pragma unroll
+            for (int j = 0; j < KPT; ++j) {
+                const uint8_t* p = kb + (t0 + TPP / CPR * j) * c.kp_s[3];
+                if constexpr (KW == 1) r.k[j] = *(const uint32_t*)p;
+                else { const u32x2 x = *(const u32x2*)p; r.k[2 * j] = x.x; r.k[2 * j + 1] = x.y; }
+            }
+        }
+        if constexpr (takes_v(up)) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint8_t* p = vb + (t0 + j) * c.vp_s[3];
+                if constexpr (VC * BITS == 16) r.v[j] = *(const uint16_t*)p;
+                else if constexpr (VW == 1) r.v[j] = *(const uint32_t*)p;
+                else { const u32x2 x = *(const u32x2*)p; r.v[2 * j] = x.x; r.v[2 * j + 1] = x.y; }
+            }
         }
     };
     auto put_k = [&](int buf, int j, u32x4 x) __attribute__((always_inline)) {
-        const int row = kPg * pg + kr + 256 / CPR * j;
-        *(u32x4*)&s_k[buf][Lds::k_at(kc & 3, row, kc >> 2)] = x;
+        *(u32x4*)&s_k[buf][Lds::k_at(kc & 3, kPg * pg + kr + TPP / CPR * j, kc >> 2)] = x;
     };
-    const int vjb = 2 * pg + (vq >> 3), vlg = vq & 3, vhalf = 8 * ((vq >> 2) & 1);
-    auto put_v = [&](int buf, int i, u32x2 x) __attribute__((always_inline)) {
-        *(u32x2*)&s_v[buf][Lds::v_at(vlg, 16 * i + vc, vjb) + vhalf] = x;
-    };
-    auto write = [&](const Raw& r, int t, int buf) __attribute__((always_inline)) {
-        const int page = 2 * t + pg;
+    const int v_to = Lds::v_at(vq & 3, vc, 2 * pg + (vq >> 3)) + 8 * ((vq >> 2) & 1);
+    auto put_v = [&](int buf, int i, u32x2 x) __attribute__((always_inline)) { *(u32x2*)&s_v[buf][v_to + 16 * i * Lds::VROW] = x; };
+    auto write_k = [&](const Raw& r, int t) __attribute__((always_inline)) {
+        const int page = 2 * t + pg, buf = t & 1;
         if (page < code_pages) {
-            constexpr float up = kCodeUp<BITS>;
-            uint32_t sk[4], mk[4];
-            const uint32_t sw[4] = {r.ks.x, r.ks.y, r.ks.z, r.ks.w}, mw[4] = {r.km.x, r.km.y, r.km.z, r.km.w};
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {        // channels u and u + 4 (INT4), 2 u and 2 u + 1 (INT8)
-                const int c0 = BITS == 4 ? u : 2 * u, c1 = BITS == 4 ? u + 4 : 2 * u + 1;
-                sk[u] = pack_h2(meta_f<MT>(sw[c0 >> 1] >> (16 * (c0 & 1))) * (up * kKExp), meta_f<MT>(sw[c1 >> 1] >> (16 * (c1 & 1))) * (up * kKExp));
-                mk[u] = pack_h2(meta_f<MT>(mw[c0 >> 1] >> (16 * (c0 & 1))) * kKExp, meta_f<MT>(mw[c1 >> 1] >> (16 * (c1 & 1))) * kKExp);
-            }
+            const u32x4 sk = *(const u32x4*)&s_km[buf][pg][0][8 * kc], mk = *(const u32x4*)&s_km[buf][pg][1][8 * kc];
 #pragma unroll
             for (int j = 0; j < KPT; ++j) {
                 uint32_t x[4];
-                key_codes<BITS>(&r.k[j][0], x);
-                put_k(buf, j, u32x4{fma_h2(x[0], sk[0], mk[0]), fma_h2(x[1], sk[1], mk[1]), fma_h2(x[2], sk[2], mk[2]), fma_h2(x[3], sk[3], mk[3])});
+                key_codes<BITS>(&r.k[j * KW], x);
+                put_k(buf, j, u32x4{fma_h2(x[0], sk.x, mk.x), fma_h2(x[1], sk.y, mk.y), fma_h2(x[2], sk.z, mk.z), fma_h2(x[3], sk.w, mk.w)});
             }
-            uint32_t sv[2], mv[2];
+        } else {                                 // the partial page, its last row repeated past the end; no keys: zeros
+            const TailArgs& tl = P.t;
+            const uint16_t* kt = (const uint16_t*)tl.k + item * tl.ks[1] + h * tl.ks[2] + 8 * kc;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                sv[u] = pack_h2(meta_f<MT>(r.vs[2 * u]) * up, meta_f<MT>(r.vs[2 * u + 1]) * up);
-                mv[u] = pack_h2(meta_f<MT>(r.vm[2 * u]), meta_f<MT>(r.vm[2 * u + 1]));
+            for (int j = 0; j < KPT; ++j) {
+                u32x4 x = {0u, 0u, 0u, 0u};
+                if (page * kPg < P.keys) x = tail_keys<BITS>(kt + (int64_t)min(kr + TPP / CPR * j, tl.len - 1) * tl.ks[3]);
+                put_k(buf, j, x);
             }
-            if (page * kPg < lo) {               // values of padding tokens count as 0, whatever they are
-                asm volatile("");
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int key = page * kPg + 4 * vq + 2 * u;
-                    const uint32_t on = (key >= lo ? 0xFFFFu : 0u) | (key + 1 >= lo ? 0xFFFF0000u : 0u);
-                    sv[u] &= on;
-                    mv[u] &= on;
-                }
-            }
+        }
+    };
+    auto write_v = [&](const Raw& r, int t) __attribute__((always_inline)) {
+        const int page = 2 * t + pg, buf = t & 1;
+        if (page < code_pages) {
+            const u32x2 sv = *(const u32x2*)&s_vm[buf][pg][vg][0][4 * vq], mv = *(const u32x2*)&s_vm[buf][pg][vg][1][4 * vq];
 #pragma unroll
             for (int i = 0; i < VC; ++i) {
                 const int d = BITS == 8 ? i >> 2 : 0;
-                put_v(buf, i, u32x2{fma_h2(value_pair<BITS>(r.v[0][d], r.v[1][d], i), sv[0], mv[0]),
-                                    fma_h2(value_pair<BITS>(r.v[2][d], r.v[3][d], i), sv[1], mv[1])});
+                put_v(buf, i, u32x2{fma_h2(value_pair<BITS>(r.v[d], r.v[VW + d], i), sv.x, mv.x),
+                                    fma_h2(value_pair<BITS>(r.v[2 * VW + d], r.v[3 * VW + d], i), sv.y, mv.y)});
             }
-        } else if (page * kPg < P.keys) {        // the partial page
+        } else {                                 // past the end: masked, and values of 0
             const TailArgs& tl = P.t;
-            const uint16_t* kt = (const uint16_t*)tl.k + item * tl.ks[1] + h * tl.ks[2] + 8 * kc;
             const uint16_t* vt = (const uint16_t*)tl.v + item * tl.vs[1] + h * tl.vs[2] + VC * vc;
-#pragma unroll
-            for (int j = 0; j < KPT; ++j)
-                put_k(buf, j, tail_keys<BITS>(kt + (int64_t)min(kr + 256 / CPR * j, tl.len - 1) * tl.ks[3]));
             uint32_t x[4][VC / 2];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int key = 4 * vq + j;
-                const bool on = key < tl.len && page * kPg + key >= lo;
-                const uint32_t* p = (const uint32_t*)(vt + (int64_t)min(key, tl.len - 1) * tl.vs[3]);
+                const int key = page * kPg + 4 * vq + j;
 #pragma unroll
-                for (int u = 0; u < VC / 2; ++u) x[j][u] = on ? p[u] : 0u;
+                for (int k = 0; k < VC / 2; ++k) x[j][k] = 0u;
+                if (key >= lo && key < P.keys) {
+                    const uint32_t* p = (const uint32_t*)(vt + (int64_t)(4 * vq + j) * tl.vs[3]);
+#pragma unroll
+                    for (int k = 0; k < VC / 2; ++k) x[j][k] = p[k];
+                }
             }
 #pragma unroll
             for (int i = 0; i < VC; ++i)
                 put_v(buf, i, u32x2{tail_pair(x[0][i >> 1], x[1][i >> 1], i & 1), tail_pair(x[2][i >> 1], x[3][i >> 1], i & 1)});
-        } else {                                 // no keys: masked, and values of 0
-#pragma unroll
-            for (int j = 0; j < KPT; ++j) put_k(buf, j, u32x4{0u, 0u, 0u, 0u});
-#pragma unroll
-            for (int i = 0; i < VC; ++i) put_v(buf, i, u32x2{0u, 0u});
         }
     };
 
@@ -810,9 +832,9 @@ void shared_tile_kernel(SharedParams a) {
 #pragma unroll
     for (int st = 0; st < NS; ++st) k_lane[st] = Lds::k_at(lg, n, st);
     const int v_lane = Lds::v_at(lg, n, 0);      // its chunk bits XORed with the key block's
-    static_assert(Lds::VPL % 64 == 0 && Lds::VROW == 64, "chunk bits are the low ones of a row");
+    static_assert(Lds::VPL % Lds::VROW == 0, "chunk bits are the low ones of a row");
 
-    // The two products of a wave's SUB keys from key `k0` of a stage on.
+    // The two products of a wave's 64 keys from key `k0` of a stage on.
     auto qk = [&](const uint8_t* sk, int k0, v4f (&s)[QB][NK]) __attribute__((always_inline)) {
 #pragma unroll
         for (int kb = 0; kb < NK; ++kb)
@@ -849,55 +871,66 @@ void shared_tile_kernel(SharedParams a) {
     const int hi_top = pi == 1 ? P.keys - a.Sq + min(wg_row0 + RT - 1, P.rows - 1) / a.G : P.keys - 1;
     const int t_begin = max(split * P.per_split, lo / kST);
     const int t_end = min(min((split + 1) * P.per_split, (P.pages + 1) / 2), hi_top / kST + 1);
-    if (t_begin < t_end) {
+    auto run = [&](auto up) __attribute__((always_inline)) {
+        constexpr bool UP = decltype(up)::value;
         Raw raw;
-        load(raw, t_begin);
-        write(raw, t_begin, 0);
-        if (t_begin + 1 < t_end) load(raw, t_begin + 1);
+        RawMeta meta = {};
+        auto write = [&](int t) __attribute__((always_inline)) {         // stage t, and what comes after it
+            if constexpr (takes_k(up)) write_k(raw, t);
+            if constexpr (takes_v(up)) write_v(raw, t);
+            put_meta(up, meta, t + 1);           // stage t - 1's place: nobody has read that since the last barrier
+            load(up, raw, t + 1);
+            load_meta(up, meta, t + 2);
+        };
+        load_meta(up, meta, t_begin);
+        load(up, raw, t_begin);
+        put_meta(up, meta, t_begin);
+        load_meta(up, meta, t_begin + 1);
+        lds_barrier();
+        write(t_begin);
         lds_barrier();
         for (int t = t_begin; t < t_end; ++t) {
-            const int buf = (t - t_begin) & 1;
-            auto next = [&]() __attribute__((always_inline)) {
-                if (t + 1 >= t_end) return;
-                write(raw, t + 1, buf ^ 1);
-                if (t + 2 < t_end) load(raw, t + 2);
-            };
-            // a SIMD's two waves (w, w + 4) take their vector-only part at opposite ends of the stage
-            if (w >= kTW / 2) next();
+            const int buf = t & 1;
+            // a SIMD's waves take their vector-only part at opposite ends of the stage
+            if (UP && t + 1 < t_end) write(t + 1);
             if (wave_on) {
                 const int k0 = kg * (kST / KG);
                 v8h pb[QB][NJ];
 #pragma unroll 1
                 for (int u = 0; u < NSUB; ++u) {
                     v4f s[QB][NK];
-                    qk(s_k[buf], k0 + SUB * u, s);
-                    const int key0 = t * kST + k0 + SUB * u;
-                    if (key0 < lo || key0 + SUB - 1 > hi_all) mask_step(s, key0 + 4 * lg, lo, hi);
+                    qk(s_k[buf], k0 + kPg * u, s);
+                    const int key0 = t * kST + k0 + kPg * u;
+                    if (key0 < lo || key0 + kPg - 1 > hi_all) mask_step(s, key0 + 4 * lg, lo, hi);
                     softmax_step(s, rs, m_run, o, ol, pb);
                     __builtin_amdgcn_sched_barrier(0);
-                    pv(s_v[buf], k0 + SUB * u, pb);
+                    pv(s_v[buf], k0 + kPg * u, pb);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if (w < kTW / 2) next();
+            if (!UP && t + 1 < t_end) write(t + 1);
             lds_barrier();
         }
+    };
+    if (t_begin < t_end) {
+        if (upper) run(std::true_type{});
+        else run(std::false_type{});
     }
 
     // The key groups' states of a row group meet in key group 0's wave.
     if constexpr (KG > 1) {
-        constexpr int NSL = QB * NT, kHalf = 2 * kST * D * 2 / 16;       // of each of the K and V buffers
+        constexpr int NSL = QB * NT, kHalf = 2 * Lds::KB / 16;       // of each of the K and V buffers
         static_assert((kTW - RG) * NSL * 64 * 16 <= 2 * kHalf * 16, "states fit the stage buffers");
         __shared__ float2 s_ml[(kTW - RG) * QB * 64];
         v4f* st0 = (v4f*)&s_k[0][0];
         v4f* st1 = (v4f*)&s_v[0][0];
-        auto slot = [&](int i) -> v4f* { return i < kHalf ? st0 + i : st1 + (i - kHalf); };
+        auto state = [&](int i) -> v4f* { return i < kHalf ? st0 + i : st1 + (i - kHalf); };
         if (kg > 0) {
             const int src = w - RG;
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
 #pragma unroll
-                for (int i = 0; i < NT; ++i) *slot((src * NSL + qb * NT + i) * 64 + L) = o[qb][i];
+                for (int i = 0; i < NT; ++i) *state((src * NSL + qb * NT + i) * 64 + L) = o[qb][i];
                 s_ml[(src * QB + qb) * 64 + L] = make_float2(m_run[qb], ol[qb][0]);
             }
         }
@@ -925,7 +958,7 @@ void shared_tile_kernel(SharedParams a) {
                 v4f t = o[qb][i] * wt[0];
 #pragma unroll
                 for (int u = 1; u < KG; ++u) {
-                    const v4f y = *slot((((u - 1) * RG + w) * NSL + qb * NT + i) * 64 + L);
+                    const v4f y = *state((((u - 1) * RG + w) * NSL + qb * NT + i) * 64 + L);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) t[r] = fmaf(wt[u], y[r], t[r]);
                 }
@@ -1040,9 +1073,9 @@ void plan_part(SharedPart& p, int Hkv, int kg, int64_t pages_a_wg) {
     p.tiles = (int)ceil_div(p.rows, rt);
     p.pages = (int)ceil_div(p.keys, kPg);
     const int64_t groups = (int64_t)p.items * Hkv * p.tiles;
-    if (kg) {       // one workgroup a CU; at least two stages each
+    if (kg) {       // one workgroup a CU; at least four pages each
         const int stages = (int)ceil_div(p.pages, 2);
-        const int64_t s = std::min(std::max<int64_t>(1, 256 / groups), ceil_div(stages, 2));
+        const int64_t s = std::min(std::max<int64_t>(1, 256 / groups), ceil_div(p.pages, 4));
         p.per_split = (int)ceil_div(stages, s);
         p.splits = (int)ceil_div(stages, p.per_split);
     } else {
@@ -1103,6 +1136,13 @@ hipError_t launch_shared_prefix(const Int4Cache& pc, const TailArgs& pt, const I
     a.p[0].c = pc; a.p[0].t = pt; a.p[0].keys = pc.S + pt.len; a.p[0].items = 1; a.p[0].rows = q.B * q.S_q * G;
     a.p[1].c = sc; a.p[1].t = st_; a.p[1].keys = sc.S + st_.len; a.p[1].items = q.B; a.p[1].rows = q.S_q * G;
     a.Hkv = pc.Hkv;
+    for (SharedPart& p : a.p) {
+        if (p.c.S) continue;
+        // no whole page: the loads that run ahead read the first query's channels, and nobody uses them
+        p.c.kp = p.c.vp = (const uint8_t*)q.q;
+        p.c.ksc = p.c.kmn = p.c.vsc = p.c.vmn = q.q;
+        for (int i = 0; i < 4; ++i) p.c.kp_s[i] = p.c.vp_s[i] = p.c.ksc_s[i] = p.c.kmn_s[i] = p.c.vsc_s[i] = p.c.vmn_s[i] = 0;
+    }
     int kg[2];
     plan_forms(a, pc.D, pc.bits, kg);
     if (!ws) {
@@ -1128,8 +1168,8 @@ hipError_t launch_shared_prefix(const Int4Cache& pc, const TailArgs& pt, const I
     }
 #define FQ_ST(D_, B_, K_)                                                                                              \
     if (pc.D == D_ && pc.bits == B_ && kg == K_) {                                                                     \
-        if (bf) hipLaunchKernelGGL((shared_tile_kernel<D_, B_, bf16, K_>), grid, dim3(64 * kTW), 0, st, a);            \
-        else hipLaunchKernelGGL((shared_tile_kernel<D_, B_, f16, K_>), grid, dim3(64 * kTW), 0, st, a);                \
+        if (bf) hipLaunchKernelGGL((shared_tile_kernel<D_, B_, bf16, K_>), grid, dim3(64 * tile_waves(K_)), 0, st, a);            \
+        else hipLaunchKernelGGL((shared_tile_kernel<D_, B_, f16, K_>), grid, dim3(64 * tile_waves(K_)), 0, st, a);                \
         return hipGetLastError();                                                                                      \
     }
 #define FQ_SPQ(D_, B_) FQ_SP(D_, B_) FQ_ST(D_, B_, 1) FQ_ST(D_, B_, 2)
