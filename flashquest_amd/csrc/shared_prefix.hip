@@ -116,18 +116,17 @@ FQ_DEV float rows_max(float v) {         // over lanes n, n + 16, n + 32, n + 48
     return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
 }
 
-// A row's query as B operands: step s holds channels base + step s .. + 7, in the order the
-// codes unpack (INT4: u, u + 4 side by side).  q times 2^-e with the largest of the row below
+// A row's query as B operands: step s holds the 8 channels of q[s], in the order the codes unpack
+// (INT4: u, u + 4 side by side).  q times 2^-e with the largest of the row below
 // 1 is exact in fp16 (16-bit inputs: what underflows is below 2^-24 of it); returns the
 // factor from S^T to scores in the log2 domain.
 template <int D, int BITS>
-FQ_DEV float load_query(const uint16_t* q, int base, int step, bool bf, float qk_scale, v8h (&qf)[D / 32]) {
+FQ_DEV float turn_query(const u32x4 (&q)[D / 32], bool bf, float qk_scale, v8h (&qf)[D / 32]) {
     float x[D / 32][8];
     float mx = 0.f;
 #pragma unroll
     for (int s = 0; s < D / 32; ++s) {
-        const u32x4 v = *(const u32x4*)(q + base + step * s);
-        const uint32_t d[4] = {v.x, v.y, v.z, v.w};
+        const uint32_t d[4] = {q[s].x, q[s].y, q[s].z, q[s].w};
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             x[s][2 * u] = bf ? bf16_bits_to_f(d[u] & 0xFFFFu) : f16_bits_to_f(d[u] & 0xFFFFu);
@@ -303,10 +302,10 @@ struct alignas(16) WaveMeta {
 FQ_DEV constexpr int slot_key(int u) { return (u & 3) + 16 * (u >> 2); }      // u = 0 .. 7, before 32 j + 4 lg
 
 // Few rows: a wave takes 16 rows and every fourth page of its workgroup's range, its loads and
-// operands its own, and the four waves' states meet in LDS.  The loads of a page are not in
-// flight during the page before: with two waves a SIMD the other wave fills the wait, and the
-// registers for a second page would leave room for one (the suffixes of 64 sequences, INT8: 24 us
-// then, 14 now; three or four waves a SIMD spill and are slower).
+// operands its own, and the four waves' states meet in LDS.  The next page's metadata, keys and
+// values are loaded into the registers of this one's as each has been used: a second set would
+// leave room for one wave a SIMD instead of two (the suffixes of 64 sequences, INT8: 24 us then,
+// 13.5 now; three or four waves a SIMD spill and are slower).
 template <int D, int BITS, typename MT>
 __global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void shared_attn_kernel(SharedParams a) {
@@ -332,6 +331,7 @@ void shared_attn_kernel(SharedParams a) {
     int hi[QB];                                  // last key a row attends
     float rs[QB];                                // S^T -> scores in the log2 domain
     v8h qf[QB][NS];
+    u32x4 qr[QB][NS];                            // turned when the first keys are on their way
     int lo = 0, hi_all = P.keys - 1;             // first key; the least hi of the tile
     if (pi == 1) {
         if (a.start) lo = min(max(a.start[item], 0), P.keys);
@@ -343,7 +343,8 @@ void shared_attn_kernel(SharedParams a) {
         const RowPlace r = row_place(row, a.G, a.Sq, pi == 1, item);
         hi[qb] = pi == 1 ? P.keys - a.Sq + r.i : P.keys - 1;
         const uint16_t* q = (const uint16_t*)a.q + r.b * a.q_s[0] + (int64_t)(h * a.G + r.g) * a.q_s[1] + r.i * a.q_s[2];
-        rs[qb] = load_query<D, BITS>(q, (D / 4) * lg, 8, a.bf16, a.qk_scale, qf[qb]);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) qr[qb][s] = *(const u32x4*)(q + (D / 4) * lg + 8 * s);
     }
 
     v4f o[QB][NT], ol[QB];
@@ -359,7 +360,7 @@ void shared_attn_kernel(SharedParams a) {
 
     // One page of 64 keys: kf(T, s) and vf(j, i) give its operands, masked: some row's keys end
     // or begin inside it.
-    auto page_step = [&](int page, bool masked, auto kf, auto vf) {
+    auto page_step = [&](int page, bool masked, auto kf, auto vf, auto k_done) __attribute__((always_inline)) {
         v4f s[QB][4];
 #pragma unroll
         for (int T = 0; T < 4; ++T) {
@@ -372,6 +373,7 @@ void shared_attn_kernel(SharedParams a) {
                 for (int qb = 0; qb < QB; ++qb) s[qb][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[qb][st], s[qb][T], 0, 0, 0);
             }
         }
+        k_done();
         if (masked) mask_step(s, page * kPg + 4 * lg, lo, hi);
         v8h pb[QB][2];
         softmax_step(s, rs, m_run, o, ol, pb);
@@ -400,7 +402,7 @@ void shared_attn_kernel(SharedParams a) {
     const uint16_t* vmb = (const uint16_t*)c.vmn + item * c.vmn_s[1] + h * c.vmn_s[2] + L * c.vmn_s[3];
     const int G = c.G;
 
-    auto load = [&](PageRaw<D, BITS>& r, int page) {
+    auto load_k = [&](PageRaw<D, BITS>& r, int page) __attribute__((always_inline)) {
         const int64_t t0 = (int64_t)page * kPg;
         const uint8_t* kp = kb + t0 * c.kp_s[3];
 #pragma unroll
@@ -417,7 +419,9 @@ void shared_attn_kernel(SharedParams a) {
                 }
             }
         }
-        const uint8_t* vp = vb + t0 * c.vp_s[3];
+    };
+    auto load_v = [&](PageRaw<D, BITS>& r, int page) __attribute__((always_inline)) {
+        const uint8_t* vp = vb + (int64_t)page * kPg * c.vp_s[3];
 #pragma unroll
         for (int u = 0; u < 16; ++u) {
             const uint8_t* p = vp + (32 * (u >> 3) + slot_key(u & 7)) * c.vp_s[3];
@@ -425,7 +429,9 @@ void shared_attn_kernel(SharedParams a) {
             else if constexpr (D * BITS == 512) r.v[u][0] = *(const uint32_t*)p;
             else { const u32x2 x = *(const u32x2*)p; r.v[u][0] = x.x; r.v[u][1] = x.y; }
         }
-        const int64_t ks = page * c.ksc_s[3], km = page * c.kmn_s[3];
+    };
+    auto load_meta = [&](PageRaw<D, BITS>& r, int page) __attribute__((always_inline)) {
+        const int64_t t0 = (int64_t)page * kPg, ks = page * c.ksc_s[3], km = page * c.kmn_s[3];
         r.ks[0] = ksb[ks + (mcl ? 0 : mc0)]; r.ks[1] = ksb[ks + (mcl ? 0 : mc1)];
         r.km[0] = kmb[km + (mcl ? 0 : mc0)]; r.km[1] = kmb[km + (mcl ? 0 : mc1)];
         const uint16_t* vs = vsb + t0 * c.vsc_s[3];
@@ -440,7 +446,7 @@ void shared_attn_kernel(SharedParams a) {
         }
     };
 
-    auto code_page = [&](const PageRaw<D, BITS>& r, int page) {
+    auto code_page = [&](PageRaw<D, BITS>& r, int page, int next) __attribute__((always_inline)) {
         // metadata through LDS: every lane converts its share, all read it in operand order
         constexpr float up = kCodeUp<BITS>;
         lds_order();
@@ -456,6 +462,7 @@ void shared_attn_kernel(SharedParams a) {
             M.vs[g][L] = on ? f_to_f16_bits(meta_f<MT>(sb) * up) : 0;
             M.vm[g][L] = on ? f_to_f16_bits(meta_f<MT>(mb)) : 0;
         }
+        if (next) load_meta(r, next);
         lds_order();
         u32x4 sk[NS], mk[NS];
 #pragma unroll
@@ -488,7 +495,10 @@ void shared_attn_kernel(SharedParams a) {
             return frag(fma_h2(x[0], sv[j][0].x, mv[j][0].x), fma_h2(x[1], sv[j][0].y, mv[j][0].y),
                         fma_h2(x[2], sv[j][1].x, mv[j][1].x), fma_h2(x[3], sv[j][1].y, mv[j][1].y));
         };
-        page_step(page, page * kPg < lo || page * kPg + kPg - 1 > hi_all, kf, vf);
+        page_step(page, page * kPg < lo || page * kPg + kPg - 1 > hi_all, kf, vf, [&]() __attribute__((always_inline)) {
+            if (next) load_k(r, next);
+        });
+        if (next) load_v(r, next);
     };
 
     // The partial page: bf16 rows, the last one repeated past the end (masked; values 0).
@@ -521,7 +531,7 @@ void shared_attn_kernel(SharedParams a) {
             }
             return frag(x[0], x[1], x[2], x[3]);
         };
-        page_step(page, true, kf, vf);
+        page_step(page, true, kf, vf, [] {});
     };
 
     // This wave's pages, every fourth of the workgroup's range; pages before the first key or
@@ -531,16 +541,24 @@ void shared_attn_kernel(SharedParams a) {
     const int p_end = min(min((split + 1) * P.per_split, P.pages), hi_top / kPg + 1);
     int page = p_first + w;
     const int code_end = min(p_end, code_pages);
+    auto turn = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) rs[qb] = turn_query<D, BITS>(qr[qb], a.bf16, a.qk_scale, qf[qb]);
+    };
     if (page < code_end) {
         PageRaw<D, BITS> r;
-        load(r, page);
+        load_meta(r, page);
+        load_k(r, page);
+        load_v(r, page);
+        turn();
         while (true) {
-            code_page(r, page);
+            const int next = page + kW < code_end ? page + kW : 0;
+            code_page(r, page, next);
             page += kW;
-            if (page >= code_end) break;
-            load(r, page);
+            if (!next) break;
         }
     }
+    if (page == p_first + w) turn();                     // (no page yet)
     if (page < p_end) tail_page(page);                   // page == code_pages: only the partial one is left
 
     // The waves' states meet in wave 0.
@@ -687,7 +705,10 @@ void shared_tile_kernel(SharedParams a) {
         const RowPlace r = row_place(row, a.G, a.Sq, pi == 1, item);
         hi[qb] = pi == 1 ? P.keys - a.Sq + r.i : P.keys - 1;
         const uint16_t* q = (const uint16_t*)a.q + r.b * a.q_s[0] + (int64_t)(h * a.G + r.g) * a.q_s[1] + r.i * a.q_s[2];
-        rs[qb] = load_query<D, BITS>(q, 8 * lg, 32, a.bf16, a.qk_scale, qf[qb]);
+        u32x4 qr[NS];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) qr[s] = *(const u32x4*)(q + 8 * lg + 32 * s);
+        rs[qb] = turn_query<D, BITS>(qr, a.bf16, a.qk_scale, qf[qb]);
     }
 
     v4f o[QB][NT], ol[QB];
