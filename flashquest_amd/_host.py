@@ -14,6 +14,8 @@ import importlib.util
 import os
 import warnings
 
+import torch
+
 from . import _lib as L
 
 _PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "_fq_host.so")
@@ -43,3 +45,10 @@ def module():
                 warnings.warn(f"the native host path is not used, build it again: {e!r}", RuntimeWarning, stacklevel=2)
         _loaded = True
     return _module
+
+
+def current():
+    """The current device and the raw stream torch launches on there.  The native calls answer None for tensors of
+    another device, so theirs is not asked for (device objects and torch.cuda's checks take a microsecond a call)."""
+    i = torch._C._cuda_getDevice()
+    return i, torch._C._cuda_getCurrentRawStream(i)

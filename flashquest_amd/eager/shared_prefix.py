@@ -67,8 +67,7 @@ def shared_prefix_attention(q: torch.Tensor, prefix: dict, suffix: dict, *, page
     """
     host = _host.module() if q.is_cuda and page_size == 64 else None
     if host is not None:
-        res = host.shared_prefix(q, prefix, suffix, suffix_start, sm_scale, bool(return_lse),
-                                 torch.cuda.current_device(), L.stream_handle(q.device))
+        res = host.shared_prefix(q, prefix, suffix, suffix_start, sm_scale, bool(return_lse), *_host.current())
         if res is not None:
             return res
     if q.dim() != 4:

@@ -141,7 +141,7 @@ def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.
     """
     host = _host.module() if q.is_cuda and page_size == 64 else None
     if host is not None:
-        out = host.rotate_append(q, k, v, cos, sin, cache, seen, torch.cuda.current_device(), L.stream_handle(q.device))
+        out = host.rotate_append(q, k, v, cos, sin, cache, seen, *_host.current())
         if out is not None:
             return out
     _check_tokens(q, k, v, cos, sin)
@@ -232,7 +232,7 @@ def dequantize_cache(cache: dict, length: int, *, start: int = 0, page_size: int
     """
     host = _host.module() if page_size == 64 else None
     if host is not None and cache.get("K_partial") is not None and cache["K_partial"].is_cuda:
-        res = host.dequantize(cache, length, start, torch.cuda.current_device(), L.stream_handle(cache["K_partial"].device))
+        res = host.dequantize(cache, length, start, *_host.current())
         if res is not None:
             return res
     bits = cache_bits(cache)
