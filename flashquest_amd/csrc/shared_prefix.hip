@@ -301,13 +301,15 @@ struct alignas(16) WaveMeta {
 // The keys of a lane's k-slots of step j of the second product: 32 j + 4 lg + {0..3}, then + 16.
 FQ_DEV constexpr int slot_key(int u) { return (u & 3) + 16 * (u >> 2); }      // u = 0 .. 7, before 32 j + 4 lg
 
+constexpr int attn_waves(int d) { return d == 64 ? 3 : 2; }      // a SIMD, as the registers allow
+
 // Few rows: a wave takes 16 rows and every fourth page of its workgroup's range, its loads and
 // operands its own, and the four waves' states meet in LDS.  The next page's metadata, keys and
 // values are loaded into the registers of this one's as each has been used: a second set would
 // leave room for one wave a SIMD instead of two (the suffixes of 64 sequences, INT8: 24 us then,
 // 13.5 now; three or four waves a SIMD spill and are slower).
 template <int D, int BITS, typename MT>
-__global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(attn_waves(D), attn_waves(D))))
 void shared_attn_kernel(SharedParams a) {
     constexpr int QB = 1;
     constexpr int NS = D / 32, NT = D / 16, RT = 16 * QB;
@@ -1106,32 +1108,37 @@ void plan_part(SharedPart& p, int Hkv, int kg, int64_t pages_a_wg) {
     p.wgs = (uint32_t)(groups * p.splits);
 }
 
-// Forms of the two parts and their plans: the least time by a model fitted to 24 .. 1024 rows
-// over 512 .. 32768 tokens (us; D = 128, INT4 / INT8 in the same words, D = 64 below):
-//   16-row waves   1.4e-3 / 1.6e-3 a page of a wave, 10 a step in all where both parts go this way
-//   row tiles      4.6 / 2.7 a stage of 256 / 128 rows on every CU, and 12 / 10 a launch for its
-//                  start, the first stage and the shares
-// 64 rows over 32768 tokens: 36 us with waves, 42 with tiles; 128 rows: 57 and 48; 512 rows over
-// 2048: 33 and 43, over 32768: 192 and 102 (tiles of 256 rows; 109 of 128).
+// Forms of the two parts and their plans: the least time by a model, in us, fitted to 80 batches (32 ..
+// 512 rows over 2048 .. 32768 tokens, suffixes of 1 and 1024, both widths and head sizes), each measured
+// in five pairs of forms; what it takes is within 1 % of the best pair on average, and at most 11 %
+// behind.  D = 128, INT4:
+//   64 rows over 32768 tokens    35 with 16-row waves, 36 and 42 with row tiles of 128 and 256
+//   128 rows                     55, 46 and 48
+//   512 rows over 2048           31, 42 and 45
+//   512 rows over 32768          174, 108 and 100
 void plan_forms(SharedParams& a, int D, int bits, int (&kg)[2]) {
-    const double wave = D == 128 ? (bits == 4 ? 1.4e-3 : 1.6e-3) : 0.9e-3;
-    const double stage[3] = {0., D == 128 ? 4.6 : 3.2, D == 128 ? 2.7 : 2.0}, start[3] = {0., 12., 10.};
-    constexpr int kSlots = 512;         // workgroups of 16-row waves that run at once
+    const int slots = 256 * attn_waves(D);       // workgroups of 16-row waves that run at once
+    constexpr double launch = 7., round = 3.2;   // a launch; a round of workgroups of 16-row waves
+    const double wave = D == 64 ? 0.65e-3 : bits == 4 ? 0.9e-3 : 1.05e-3;                // a page of a 16-row wave
+    const double first[3] = {0., 7., 4.};       // a row tile's start and shares, a stage of it
+    const double stage[3] = {0., D == 128 ? 3.7 : 2.9, D == 128 ? 2.1 : 1.6};
     double best = 0.;
     SharedPart plan[2];
     for (int k0 = 0; k0 < 3; ++k0)
         for (int k1 = 0; k1 < 3; ++k1) {
             SharedPart p[2] = {a.p[0], a.p[1]};
             const int k[2] = {k0, k1};
-            double pages = 0., t = k0 == k1 ? 0. : 5.;      // pages of 16-row waves; another launch
+            int64_t pages = 0, wgs = 0;          // of 16-row waves
             for (int i = 0; i < 2; ++i)
-                if (!k[i]) pages += (double)p[i].items * a.Hkv * ceil_div(p[i].rows, 16) * ceil_div(p[i].keys, kPg);
-            const int64_t each = std::max<int64_t>(kW, ceil_div((int64_t)pages, kSlots));
+                if (!k[i]) pages += p[i].items * a.Hkv * ceil_div(p[i].rows, 16) * ceil_div(p[i].keys, kPg);
+            const int64_t each = std::max<int64_t>(1, ceil_div(pages, kW * slots)) * kW;         // the waves take as many
+            double t = (k0 == k1 ? 1 : 2) * launch + (double)pages * wave;
             for (int i = 0; i < 2; ++i) {
                 plan_part(p[i], a.Hkv, k[i], each);
-                if (k[i]) t += (i == 1 && k0 == k1 ? 0. : start[k[i]]) + (double)ceil_div(p[i].wgs, 256) * p[i].per_split * stage[k[i]];
+                if (k[i]) t += (double)ceil_div(p[i].wgs, 256) * (p[i].per_split * stage[k[i]] + first[k[i]]);
+                else wgs += p[i].wgs;
             }
-            t += pages * wave;
+            if (wgs) t += round * std::max(1., (double)wgs / slots);
             if (best == 0. || t < best) {
                 best = t;
                 kg[0] = k0; kg[1] = k1;
