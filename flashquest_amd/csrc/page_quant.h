@@ -126,10 +126,12 @@ FQ_DEV void store_codes(uint8_t* row, int c8, const uint32_t (&c)[8]) {
     }
 }
 
-// Page pg of batch * head bh.  DT: the type of K and V, which share it; load_k(pos, c8, x):
-// channels 8 c8 .. + 7 of the key at a position, as floats.
-template <int D, int BITS, int DT, typename LoadK>
-FQ_DEV void quant_page(const PageQuantParams& a, int pg, int bh, LoadK load_k) {
+// Page pg of batch * head bh.  DT: the type of K and V, which share it; load_k(u, pos, c8, x),
+// load_v: channels 8 c8 .. + 7 of the token at a position, the thread's u-th, as floats.
+// The rows of a thread are RPP apart, and a row's address is the one before it and a uniform
+// step: 64-bit products per row and lane cost as much as the quantisation itself.
+template <int D, int BITS, int DT, typename LoadK, typename LoadV>
+FQ_DEV void quant_page(const PageQuantParams& a, int pg, int bh, LoadK load_k, LoadV load_v) {
     constexpr int CPR = D / 8;                  // threads per token row
     constexpr int RPP = kThreads / CPR;         // token rows per pass
     constexpr int TPT = kPage / RPP;            // tokens per thread
@@ -151,7 +153,7 @@ FQ_DEV void quant_page(const PageQuantParams& a, int pg, int bh, LoadK load_k) {
         float x[TPT][8];
         float mn[8], mx[8];
 #pragma unroll
-        for (int u = 0; u < TPT; ++u) load_k(lpos[u], c8, x[u]);
+        for (int u = 0; u < TPT; ++u) load_k(u, lpos[u], c8, x[u]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) { mn[i] = INFINITY; mx[i] = -INFINITY; }
 #pragma unroll
@@ -175,22 +177,28 @@ FQ_DEV void quant_page(const PageQuantParams& a, int pg, int bh, LoadK load_k) {
             for (int i = 0; i < 8; ++i) { s_red[w][c8][i] = mn[i]; s_red[w][c8][8 + i] = mx[i]; }
         }
         __syncthreads();
+        // one thread a channel: every row of threads doing it for its own eight was a third of the
+        // vector instructions of K
+        __shared__ __attribute__((aligned(16))) float s_ch[3][D];        // minimum, scale, its reciprocal
+        if (tid < D) {
+            float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
-        for (int ww = 0; ww < kThreads / 64; ++ww) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                mn[i] = fminf(mn[i], s_red[ww][c8][i]);
-                mx[i] = fmaxf(mx[i], s_red[ww][c8][8 + i]);
+            for (int ww = 0; ww < kThreads / 64; ++ww) {
+                lo = fminf(lo, s_red[ww][tid >> 3][tid & 7]);
+                hi = fmaxf(hi, s_red[ww][tid >> 3][8 + (tid & 7)]);
             }
+            // scale in the input dtype (kv_quant.py:131-149), as quant_k_kernel
+            const float diff = round_to(hi - lo, DT);
+            float sc = round_to(diff * (BITS == 8 ? kCacheInv255 : kCacheInv15), DT);
+            sc = round_to(fmaxf(sc, kCacheEps), DT);
+            s_ch[0][tid] = lo;
+            s_ch[1][tid] = sc;
+            s_ch[2][tid] = __fdiv_rn(1.0f, sc);
         }
-        // scale in the input dtype (kv_quant.py:131-149), as quant_k_kernel
-        float sc[8];
+        __syncthreads();
+        float sc[8], rc[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float diff = round_to(mx[i] - mn[i], DT);
-            float s = round_to(diff * (BITS == 8 ? kCacheInv255 : kCacheInv15), DT);
-            sc[i] = round_to(fmaxf(s, kCacheEps), DT);
-        }
+        for (int i = 0; i < 8; ++i) { mn[i] = s_ch[0][8 * c8 + i]; sc[i] = s_ch[1][8 * c8 + i]; rc[i] = s_ch[2][8 * c8 + i]; }
         if (r == 0) {
             const int64_t p = a.tok_dst0 / kPage + pg;
             uint32_t sw[4], mw[4];
@@ -209,14 +217,11 @@ FQ_DEV void quant_page(const PageQuantParams& a, int pg, int bh, LoadK load_k) {
                 make_uint4(mw[0], mw[1], mw[2], mw[3]);
         }
         if (a.k_codes) {
-            float rc[8];
             bool fine = true;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                rc[i] = __fdiv_rn(1.0f, sc[i]);
-                fine &= sc[i] <= 1e30f;
-            }
+            for (int i = 0; i < 8; ++i) fine &= sc[i] <= 1e30f;
             const bool wide = quot_wide(fine);
+            uint8_t* row = a.kp + b * a.kp_s[0] + h * a.kp_s[1] + (int64_t)(a.tok_dst0 + pg * kPage + r) * a.kp_s[2];
 #pragma unroll
             for (int u = 0; u < TPT; ++u) {
                 uint32_t cd[8];
@@ -228,8 +233,7 @@ FQ_DEV void quant_page(const PageQuantParams& a, int pg, int bh, LoadK load_k) {
                     for (int i = 0; i < 8; ++i) cd[i] = quot_code<BITS>(x[u][i] - mn[i], sc[i], rc[i]);
                 }
                 if (!ok[u]) continue;
-                store_codes<BITS>(a.kp + b * a.kp_s[0] + h * a.kp_s[1] + (int64_t)(a.tok_dst0 + pos[u]) * a.kp_s[2],
-                                  c8, cd);
+                store_codes<BITS>(row + u * (RPP * a.kp_s[2]), c8, cd);
             }
         }
     }
@@ -237,9 +241,12 @@ FQ_DEV void quant_page(const PageQuantParams& a, int pg, int bh, LoadK load_k) {
     if (a.do_v) {
         const int lpg = a.v_group / 8;          // lanes per V group (a power of two <= CPR)
         const int g = (8 * c8) / a.v_group;
+        const int64_t t0 = a.tok_dst0 + pg * kPage + r;
+        uint8_t* row = a.vp + b * a.vp_s[0] + h * a.vp_s[1] + t0 * a.vp_s[2];
+        const int64_t s0 = b * a.vs_s[0] + h * a.vs_s[1] + t0 * a.vs_s[2] + g, m0 = b * a.vm_s[0] + h * a.vm_s[1] + t0 * a.vm_s[2] + g;
         float x[TPT][8];
 #pragma unroll
-        for (int u = 0; u < TPT; ++u) load8<DT>(a.v, b, h, lpos[u], c8, x[u]);
+        for (int u = 0; u < TPT; ++u) load_v(u, lpos[u], c8, x[u]);
 #pragma unroll
         for (int u = 0; u < TPT; ++u) {
             // every lane of the row takes part in the reductions; invalid tokens are not stored
@@ -260,12 +267,11 @@ FQ_DEV void quant_page(const PageQuantParams& a, int pg, int bh, LoadK load_k) {
                 for (int i = 0; i < 8; ++i) cd[i] = quot_code<BITS>(x[u][i] - mn, s, rc);
             }
             if (!ok[u]) continue;
-            const int64_t t = a.tok_dst0 + pos[u];
             if (c8 % lpg == 0) {
-                store_any(a.vs, a.meta_dtype, b * a.vs_s[0] + h * a.vs_s[1] + t * a.vs_s[2] + g, s);
-                store_any(a.vm, a.meta_dtype, b * a.vm_s[0] + h * a.vm_s[1] + t * a.vm_s[2] + g, mn);
+                store_any(a.vs, a.meta_dtype, s0 + u * (RPP * a.vs_s[2]), s);
+                store_any(a.vm, a.meta_dtype, m0 + u * (RPP * a.vm_s[2]), mn);
             }
-            store_codes<BITS>(a.vp + b * a.vp_s[0] + h * a.vp_s[1] + t * a.vp_s[2], c8, cd);
+            store_codes<BITS>(row + u * (RPP * a.vp_s[2]), c8, cd);
         }
     }
 }

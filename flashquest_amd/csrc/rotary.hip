@@ -17,8 +17,14 @@
 //          page, so after its last load it also stages what stays in the partial page.
 //   rows   without a completed page, the new rows of K (rotated) and V to the partial page.
 //   q      the query rows.
-// All are bound by memory: every input is read once (cos / sin once per group of heads from
-// HBM, after that from the L2) and every output written once.
+// All are bound by memory: every input is read once and every output written once, the angles
+// by every head, for which the heads of a page or of a chunk of query rows run on one XCD (from
+// its L2: 5 % of a long prompt).  A thread turns
+// its query unit for 4 heads with one load of the angles; a short step, which would not fill the
+// GPU so, for one (2^19 units: 8 waves a SIMD).  32768 tokens of 24 query and 8 KV heads of 128
+// channels to an empty INT4 cache: 139 us for 0.61 GB (4.4 TB/s; a copy 5.2), of which the query
+// rows run at 5.3; the pages' vector instructions, half of the time, are what keeps them below.
+// One token: 3 us, the launch.
 #include "fq_common.h"
 #include "page_quant.h"
 
@@ -52,10 +58,24 @@ FQ_DEV void ld8(const void* p, int64_t e, float (&x)[8]) {
 template <int DT>
 FQ_DEV void st8(void* p, int64_t e, const float (&x)[8]) {
     uint32_t w[4];
+    if constexpr (DT == FQ_BF16) {
+        // the conversion instruction, of two values at once: it agrees with f_to_bf16_bits on every
+        // float but NaNs, whose payload it keeps
+        typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+        bool nan = false;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        w[i] = DT == FQ_BF16 ? (uint32_t)f_to_bf16_bits(x[2 * i]) | (uint32_t)f_to_bf16_bits(x[2 * i + 1]) << 16
-                             : (uint32_t)f_to_f16_bits(x[2 * i]) | (uint32_t)f_to_f16_bits(x[2 * i + 1]) << 16;
+        for (int i = 0; i < 4; ++i) {
+            w[i] = __builtin_bit_cast(uint32_t, bf2{(__bf16)x[2 * i], (__bf16)x[2 * i + 1]});
+            nan |= __builtin_isunordered(x[2 * i], x[2 * i + 1]);
+        }
+        if (__builtin_amdgcn_ballot_w64(nan)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = (uint32_t)f_to_bf16_bits(x[2 * i]) | (uint32_t)f_to_bf16_bits(x[2 * i + 1]) << 16;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)f_to_f16_bits(x[2 * i]) | (uint32_t)f_to_f16_bits(x[2 * i + 1]) << 16;
+    }
     *(uint4*)((char*)p + e * 2) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -97,6 +117,52 @@ FQ_DEV void rotate_pair(float (&x)[8], float (&y)[8], const Angles<CT>& a) {
     }
 }
 
+// Blocks whose tokens share angles go to one XCD, one after another, so that its L2 has them: block
+// ids go round the 8 XCDs, so items (heads) of chunk c get ids that are c modulo 8.
+constexpr int kXcd = 8;
+FQ_DEV void by_xcd(int64_t blk, int items, int& chunk, int& item) {
+    const uint32_t local = (uint32_t)(blk / kXcd);
+    chunk = (int)(local / items) * kXcd + (int)(blk % kXcd);
+    item = (int)(local % items);
+}
+int64_t xcd_blocks(int64_t chunks, int64_t items) { return (chunks + kXcd - 1) / kXcd * kXcd * items; }
+
+// One thread's share of Rows: unit u of token t (of n) for HPT heads from h0 on, rotated, all loads
+// before the first store.
+template <int DT, int CT, int HPT>
+FQ_DEV void turn_heads(const Rows& w, const Rotary& r, int b, int t, int u, int h0) {
+    int lo, hi;
+    unit_channels<DT>(r, u, lo, hi);
+    const bool turn = u < (r.R >> 4);
+    Angles<CT> ang;
+    if (turn) load_angles<CT>(r, b, w.src_t0 + t, lo, hi, ang);
+    const uint16_t* in = (const uint16_t*)w.src + b * w.ss[0] + (int64_t)(w.src_t0 + t) * w.ss[2];
+    uint16_t* out = (uint16_t*)w.dst + b * w.ds[0] + (int64_t)(w.dst_t0 + t) * w.ds[2];
+    uint4 x[HPT], y[HPT];
+#pragma unroll
+    for (int i = 0; i < HPT; ++i) {
+        const uint16_t* p = in + min(h0 + i, w.H - 1) * w.ss[1];
+        x[i] = *(const uint4*)(p + lo);
+        y[i] = *(const uint4*)(p + hi);
+    }
+#pragma unroll
+    for (int i = 0; i < HPT; ++i) {
+        if (h0 + i >= w.H) break;
+        uint16_t* p = out + (h0 + i) * w.ds[1];
+        if (turn) {
+            float xf[8], yf[8];
+            ld8<DT>(&x[i], 0, xf);
+            ld8<DT>(&y[i], 0, yf);
+            rotate_pair<CT>(xf, yf, ang);
+            st8<DT>(p, lo, xf);
+            st8<DT>(p, hi, yf);
+        } else {
+            *(uint4*)(p + lo) = x[i];
+            *(uint4*)(p + hi) = y[i];
+        }
+    }
+}
+
 // One thread's share of Rows: unit u of token t (of n + zero) for heads h0 .. h1 - 1.
 template <int DT, int CT, bool ROT>
 FQ_DEV void do_rows(const Rows& w, const Rotary& r, int b, int t, int u, int h0, int h1) {
@@ -129,14 +195,26 @@ FQ_DEV void do_rows(const Rows& w, const Rotary& r, int b, int t, int u, int h0,
 }
 
 // Threads of a Rows: (b, group of `hpt` heads, token, unit), units fastest.
-struct RowGrid { int hpt, groups; int64_t threads; };
+// chunks > 0 (many tokens, rotated, none set to 0): a block per (chunk of tokens, batch, group of 4
+// heads) instead, placed by by_xcd.
+struct RowGrid { int hpt, groups; int64_t threads; int chunks; };
 RowGrid row_grid(const Rows& w, int B, int D, int hpt) {
-    RowGrid g{hpt, (w.H + hpt - 1) / hpt, 0};
+    RowGrid g{hpt, (w.H + hpt - 1) / hpt, 0, 0};
     g.threads = (int64_t)B * g.groups * (w.n + w.zero) * (D / 16);
     return g;
 }
 template <int D, int DT, int CT, bool ROT>
 FQ_DEV void rows_block(const Rows& w, const Rotary& r, const RowGrid& g, int64_t block) {
+    if constexpr (ROT) {
+        if (g.chunks > 0) {
+            constexpr int TPB = kThreads / (D / 16);     // tokens of a block
+            int chunk, item;
+            by_xcd(block, (int)g.threads, chunk, item);
+            const int t = chunk * TPB + threadIdx.x / (D / 16);
+            if (t < w.n) turn_heads<DT, CT, 4>(w, r, item / g.groups, t, threadIdx.x % (D / 16), item % g.groups * 4);
+            return;
+        }
+    }
     const int64_t i = block * kThreads + threadIdx.x;
     if (i >= g.threads) return;
     const int u = (int)(i % (D / 16));
@@ -183,15 +261,65 @@ FQ_DEV void load8_rotated(const TokSrc& s, const Rotary& r, int b, int h, int po
     }
 }
 
+// A page of new tokens only: the thread's rows at a pointer and uniform steps.
+template <int D, int DT, int CT>
+struct FreshPage {
+    static constexpr int RPP = kThreads / (D / 8);       // rows between a thread's
+    const uint16_t *k, *v;               // the thread's first row, its channels
+    const void *cos, *sin;
+    int64_t ce, se;                      // element offsets of its first row's angles
+    int other;                           // channels to the partners
+    bool turn;
+    uint32_t flip;                       // sign bits of the partners' products
+
+    FQ_DEV FreshPage(const RotAppendParams& a, int pg, int b, int h) {
+        const TokSrc &ks = a.pq.k, &vs = a.pq.v;
+        const int c8 = threadIdx.x % (D / 8), t = pg * kPage - ks.head_len + threadIdx.x / (D / 8), ch = 8 * c8, half = a.r.R >> 1;
+        k = (const uint16_t*)ks.tail + b * ks.ts[0] + h * ks.ts[1] + t * ks.ts[2] + ch;
+        v = (const uint16_t*)vs.tail + b * vs.ts[0] + h * vs.ts[1] + t * vs.ts[2] + ch;
+        turn = ch < a.r.R;
+        other = turn ? (ch < half ? half : -half) : 0;
+        flip = ch < half ? 0x80008000u : 0u;
+        cos = a.r.cos; sin = a.r.sin;
+        ce = b * a.r.cs[0] + t * a.r.cs[1] + (turn ? ch : 0);        // (unrotated channels: loads without a use)
+        se = b * a.r.ss[0] + t * a.r.ss[1] + (turn ? ch : 0);
+    }
+    FQ_DEV void key(const RotAppendParams& a, int u, float (&x)[8]) const {
+        const uint16_t* p = k + u * (RPP * a.pq.k.ts[2]);
+        uint4 y4 = *(const uint4*)(p + other);
+        float y[8], c[8], s[8];
+        ld8<DT>(p, 0, x);
+        ld8<CT>(cos, ce + u * (RPP * a.r.cs[1]), c);
+        ld8<CT>(sin, se + u * (RPP * a.r.ss[1]), s);
+        y4 = make_uint4(y4.x ^ flip, y4.y ^ flip, y4.z ^ flip, y4.w ^ flip);
+        ld8<DT>(&y4, 0, y);
+        if (!turn) return;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float z = x[i] * c[i] + y[i] * s[i];
+            x[i] = DT == FQ_BF16 ? (float)(__bf16)z : (float)(_Float16)z;    // (a NaN stays one)
+        }
+    }
+    FQ_DEV void value(const RotAppendParams& a, int u, float (&x)[8]) const { ld8<DT>(v + u * (RPP * a.pq.v.ts[2]), 0, x); }
+};
+
 template <int D, int BITS, int DT, int CT>
 __global__ __launch_bounds__(kThreads) void rotate_append_kernel(RotAppendParams a) {
     int64_t blk = blockIdx.x;
     if (blk < a.page_blocks) {
-        const int pg = (int)(blk % a.pages), bh = (int)(blk / a.pages);
+        int pg, bh;
+        by_xcd(blk, a.pq.B * a.pq.H, pg, bh);
+        if (pg >= a.pages) return;
         const int b = bh / a.pq.H, h = bh % a.pq.H;
-        quant_page<D, BITS, DT>(a.pq, pg, bh, [&](int pos, int c8, float (&x)[8]) {
-            load8_rotated<DT, CT>(a.pq.k, a.r, b, h, pos, c8, x);
-        });
+        if (pg > 0 || a.pq.k.head_len == 0) {            // no token of the partial page
+            const FreshPage<D, DT, CT> f(a, pg, b, h);
+            quant_page<D, BITS, DT>(a.pq, pg, bh, [&](int u, int, int, float (&x)[8]) { f.key(a, u, x); },
+                                    [&](int u, int, int, float (&x)[8]) { f.value(a, u, x); });
+        } else {
+            quant_page<D, BITS, DT>(a.pq, pg, bh, [&](int, int pos, int c8, float (&x)[8]) {
+                load8_rotated<DT, CT>(a.pq.k, a.r, b, h, pos, c8, x);
+            }, [&](int, int pos, int c8, float (&x)[8]) { load8<DT>(a.pq.v, b, h, pos, c8, x); });
+        }
         if (pg == 0 && a.k.n + a.k.zero > 0) {
             __syncthreads();             // every thread has its rows of the old partial page
             const int units = D / 16, rows = a.k.n + a.k.zero;
@@ -226,7 +354,8 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateParams a) {
 // Tokens [start, S + tail) of a cache as values: code * scale + min in fp32 (an exact product,
 // one rounding), rounded to bf16 (dequantize_k_int4 / dequantize_v_int4, kv_quant.py:174-215;
 // dequantize_k / dequantize_v, 64-97), the partial page's rows as they are.  One workgroup
-// per (page, batch * head) and one thread per 8 channels, as quant_page: bound by the bytes.
+// per (page, batch * head) and one thread per 8 channels, as quant_page: bound by the bytes,
+// 32768 tokens of 8 heads of 128 channels in INT4 31 us (0.17 GB, 5.5 TB/s).
 struct DequantParams {
     Int4Cache c;
     TailArgs t;                          // 16-bit rows of the outputs' type (bf16)
@@ -293,7 +422,15 @@ __global__ __launch_bounds__(kThreads) void dequant_cache_kernel(DequantParams a
 
 // Heads a thread rotates with one load of its angles: 4 once one head a thread gives more
 // waves than the GPU holds, so that short steps keep every lane busy.
-int heads_per_thread(int64_t B, int64_t H, int64_t n, int D) { return B * H * n * (D / 16) >= (1 << 19) ? 4 : 1; }
+RowGrid rotated_grid(const Rows& w, int B, int D) {
+    const bool many = (int64_t)B * w.H * w.n * (D / 16) >= (1 << 19);
+    RowGrid g = row_grid(w, B, D, many ? 4 : 1);
+    if (many) {
+        g.chunks = (w.n + kThreads / (D / 16) - 1) / (kThreads / (D / 16));
+        g.threads = (int64_t)B * g.groups;       // items of a chunk
+    }
+    return g;
+}
 
 Rotary rotary_of(const fq_rotary& f) {
     Rotary r{};
@@ -303,7 +440,7 @@ Rotary rotary_of(const fq_rotary& f) {
     return r;
 }
 
-int64_t blocks_of(const RowGrid& g) { return (g.threads + kThreads - 1) / kThreads; }
+int64_t blocks_of(const RowGrid& g) { return g.chunks > 0 ? xcd_blocks(g.chunks, g.threads) : (g.threads + kThreads - 1) / kThreads; }
 
 template <typename F>
 hipError_t by_type(int D, int dt, int ct, F f) {
@@ -328,7 +465,7 @@ hipError_t launch_rotate_append(const Int4Cache& c, int layer, void* kpart, cons
     RotAppendParams a{};
     a.r = rotary_of(f);
     a.pages = pl.n_complete;
-    a.page_blocks = (int64_t)pl.n_complete * c.B * c.Hkv;
+    a.page_blocks = xcd_blocks(pl.n_complete, (int64_t)c.B * c.Hkv);
     if (pl.n_complete > 0) {
         PageQuantParams& p = a.pq;
         p.k = stream_src(kpart, kpart_s, l, knew, kn_s, pl.partial_len, dtype);
@@ -369,7 +506,7 @@ hipError_t launch_rotate_append(const Int4Cache& c, int layer, void* kpart, cons
     q.H = f.H_q; q.n = S_new;
     a.gk = row_grid(a.k, c.B, c.D, 1);
     a.gv = row_grid(a.v, c.B, c.D, 1);
-    a.gq = row_grid(q, c.B, c.D, heads_per_thread(c.B, f.H_q, S_new, c.D));
+    a.gq = rotated_grid(q, c.B, c.D);
     a.k_blocks = done ? 0 : blocks_of(a.gk);
     a.v_blocks = done ? 0 : blocks_of(a.gv);
     const int64_t blocks = a.page_blocks + a.k_blocks + a.v_blocks + blocks_of(a.gq);
@@ -395,7 +532,7 @@ hipError_t launch_rotate(const fq_rotary& f, const void* k, const int64_t* k_s, 
     };
     a.x[0] = rows(f.q, f.q_strides, f.q_out, f.qo_strides, f.H_q);
     a.x[1] = rows(k, k_s, k_out, ko_s, H_kv);
-    for (int i = 0; i < 2; ++i) a.g[i] = row_grid(a.x[i], B, D, heads_per_thread(B, a.x[i].H, S, D));
+    for (int i = 0; i < 2; ++i) a.g[i] = rotated_grid(a.x[i], B, D);
     a.blocks0 = blocks_of(a.g[0]);
     const int64_t blocks = a.blocks0 + blocks_of(a.g[1]);
     if (blocks == 0) return hipSuccess;
