@@ -1503,7 +1503,8 @@ static int check_shared(const fq_int4_cache* prefix, const fq_tail* prefix_tail,
     if (pc.S + pt.len < 1) return fail(FQ_ERR_INVALID, "the prefix has no tokens");
     if (q->S_q < 1 || sc.S + st_.len < q->S_q)
         return fail(FQ_ERR_INVALID, "S_q=%d query tokens, the suffix has %d (they are its last)", q->S_q, sc.S + st_.len);
-    if ((int64_t)q->B * q->H_q * q->S_q > 0x7FFFFFFF / 64) return fail(FQ_ERR_UNSUPPORTED, "too many query rows");
+    if ((int64_t)q->B * q->H_q * q->S_q > 1 << 21)       // the grids hold that many rows in every form
+        return fail(FQ_ERR_UNSUPPORTED, "%lld query rows (at most 2097152 a call)", (long long)q->B * q->H_q * q->S_q);
     if (!is_half(q->dtype)) return fail(FQ_ERR_UNSUPPORTED, "queries must be bf16 or fp16");
     if (pc.S == 0) pc.meta_dtype = sc.meta_dtype;
     if (!pointers) return FQ_OK;

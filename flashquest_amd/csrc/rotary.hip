@@ -511,7 +511,7 @@ hipError_t launch_rotate_append(const Int4Cache& c, int layer, void* kpart, cons
     a.v_blocks = done ? 0 : blocks_of(a.gv);
     const int64_t blocks = a.page_blocks + a.k_blocks + a.v_blocks + blocks_of(a.gq);
     if (blocks == 0) return hipSuccess;
-    if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+    if (blocks * kThreads > 0xFFFFFFFFll) return hipErrorInvalidValue;
     return by_type(c.D, dtype, f.dtype, [&](auto D, auto DT, auto CT) {
         if (c.bits == 8) hipLaunchKernelGGL((rotate_append_kernel<D(), 8, DT(), CT()>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a);
         else hipLaunchKernelGGL((rotate_append_kernel<D(), 4, DT(), CT()>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a);
@@ -536,7 +536,7 @@ hipError_t launch_rotate(const fq_rotary& f, const void* k, const int64_t* k_s, 
     a.blocks0 = blocks_of(a.g[0]);
     const int64_t blocks = a.blocks0 + blocks_of(a.g[1]);
     if (blocks == 0) return hipSuccess;
-    if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+    if (blocks * kThreads > 0xFFFFFFFFll) return hipErrorInvalidValue;
     return by_type(D, dtype, f.dtype, [&](auto D_, auto DT, auto CT) {
         hipLaunchKernelGGL((rotate_kernel<D_(), DT(), CT()>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a);
         return hipGetLastError();

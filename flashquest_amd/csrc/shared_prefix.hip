@@ -279,6 +279,45 @@ FQ_DEV void mask_step(v4f (&s)[QB][NK], int key0, int lo, const int (&hi)[QB]) {
             }
 }
 
+// Values that are not finite, where a sequence has several query tokens: a weight of 0 times one is
+// not 0, so rows that end before it would not be free of it.  Such values are taken as 0, and rows
+// that give them a weight get NaN.  It costs 3 to 8 % of the row tiles' time (their registers).  (Keys that are not finite need none of this: scores of keys that
+// a row does not attend are replaced.)
+//
+// 0xFFFF for each half where the scale or the minimum is not finite (fp16).
+FQ_DEV uint32_t not_finite(uint32_t s, uint32_t m) {
+    typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+    const us2 x = __builtin_elementwise_max(__builtin_bit_cast(us2, s & 0x7FFF7FFFu), __builtin_bit_cast(us2, m & 0x7FFF7FFFu));
+    return (x.x >= 0x7C00u ? 0xFFFFu : 0u) | (x.y >= 0x7C00u ? 0xFFFF0000u : 0u);
+}
+// Whether any of 2 N bf16 values is not finite in fp16.
+template <int N>
+FQ_DEV uint32_t tail_not_finite(const uint32_t (&x)[N]) {
+    uint32_t b = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) b |= (x[k] & 0x7FFFu) >= 0x4780u || (x[k] & 0x7FFF0000u) >= 0x47800000u;     // 2^16 and more
+    return b;
+}
+// bad[T]: such masks of the lane's keys 16 T + 4 lg + {0, 1}, {2, 3}; pb: the weights.
+template <int QB, int NT>
+FQ_DEV void spoil_rows(const u32x2 (&bad)[4], const v8h (&pb)[QB][2], v4f (&o)[QB][NT]) {
+    uint32_t hit[QB], any = 0;
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        const u32x4 p = __builtin_bit_cast(u32x4, pb[qb][0]), q = __builtin_bit_cast(u32x4, pb[qb][1]);
+        hit[qb] = (p.x & bad[0].x) | (p.y & bad[0].y) | (p.z & bad[1].x) | (p.w & bad[1].y) |
+                  (q.x & bad[2].x) | (q.y & bad[2].y) | (q.z & bad[3].x) | (q.w & bad[3].y);
+        any |= hit[qb];
+    }
+    if (!__builtin_amdgcn_ballot_w64(any != 0)) return;
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        const float x = rows_max(hit[qb] ? 1.f : 0.f) > 0.f ? NAN : 0.f;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) o[qb][i] += x;
+    }
+}
+
 // A page as it is in memory: one lane's K bytes of keys 16 T + n (channels D/4 lg ..) and V
 // bytes of 16 keys (channels D/16 n ..), and its share of the page's metadata.
 template <int D, int BITS>
@@ -296,6 +335,7 @@ template <int D>
 struct alignas(16) WaveMeta {
     uint16_t ks[D], km[D];
     uint16_t vs[4][kPg], vm[4][kPg];
+    uint16_t bad[kPg];                   // spoil_rows' masks
 };
 
 // The keys of a lane's k-slots of step j of the second product: 32 j + 4 lg + {0..3}, then + 16.
@@ -360,6 +400,8 @@ void shared_attn_kernel(SharedParams a) {
     }
     const v8h ones = frag(0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u);
 
+    const bool several = pi == 1 && a.Sq > 1;    // rows of several query tokens
+
     // One page of 64 keys: kf(T, s) and vf(j, i) give its operands, masked: some row's keys end
     // or begin inside it.
     auto page_step = [&](int page, bool masked, auto kf, auto vf, auto k_done) __attribute__((always_inline)) {
@@ -389,6 +431,13 @@ void shared_attn_kernel(SharedParams a) {
             }
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) ol[qb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pb[qb][j], ol[qb], 0, 0, 0);
+        }
+        if (several) {
+            asm volatile("");
+            u32x2 bad[4];
+#pragma unroll
+            for (int T = 0; T < 4; ++T) bad[T] = *(const u32x2*)&M.bad[16 * T + 4 * lg];
+            spoil_rows(bad, pb, o);
         }
     };
 
@@ -456,7 +505,19 @@ void shared_attn_kernel(SharedParams a) {
             *(uint32_t*)&M.ks[2 * L] = pack_h2(meta_f<MT>(r.ks[0]) * (up * kKExp), meta_f<MT>(r.ks[1]) * (up * kKExp));
             *(uint32_t*)&M.km[2 * L] = pack_h2(meta_f<MT>(r.km[0]) * kKExp, meta_f<MT>(r.km[1]) * kKExp);
         }
-        const bool on = page * kPg + L >= lo;            // values of padding tokens count as 0, whatever they are
+        bool on = page * kPg + L >= lo;                  // values of padding tokens count as 0, whatever they are
+        if (several) {
+            asm volatile("");
+            bool fine = true;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                if (g >= G) break;
+                const uint32_t sb = (g < 2 ? r.vs.x : r.vs.y) >> (16 * (g & 1)), mb = (g < 2 ? r.vm.x : r.vm.y) >> (16 * (g & 1));
+                fine &= fabsf(meta_f<MT>(sb)) * up < 65520.f && fabsf(meta_f<MT>(mb)) < 65520.f;         // finite in fp16; false for NaN
+            }
+            M.bad[L] = on && !fine ? 0xFFFFu : 0u;
+            on = on && fine;
+        }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             if (g >= G) break;
@@ -524,6 +585,20 @@ void shared_attn_kernel(SharedParams a) {
                 const u32x2 x = *(const u32x2*)p;
                 tv[u][0] = on ? x.x : 0u; tv[u][1] = on ? x.y : 0u;
             }
+        }
+        if (several) {
+            asm volatile("");
+            lds_order();
+            M.bad[L] = 0;
+            lds_order();
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                const uint32_t b = tail_not_finite(tv[u]);
+                if (b) M.bad[32 * (u >> 3) + slot_key(u & 7) + 4 * lg] = 0xFFFFu;        // (any lane that has one)
+#pragma unroll
+                for (int k = 0; k < NT / 2; ++k) tv[u][k] = b ? 0u : tv[u][k];
+            }
+            lds_order();
         }
         auto vf = [&](int j, int i) {
             uint32_t x[4];
@@ -632,6 +707,9 @@ void shared_attn_kernel(SharedParams a) {
 // other waves have work while one waits.  512 rows over 32768 tokens in INT4: 102 us with 8 waves for
 // KG = 1, 106 with 16; 128 rows: 49 with 8 for KG = 2, 47 with 16; 320 rows over 16384: 60 and 49.
 //
+// SEVERAL: a launch with suffixes of several query tokens (spoil_rows); without it a step of one token
+// is 1 to 2 % faster.
+//
 // LDS holds a plane for each lane group lg of the operands: K's plane has a row per key of the
 // chunks (8 channels, 16 bytes) 4 st + lg, V's a row per channel of the chunks (8 keys) 4 jb + lg.
 // A 16-byte read of 64 lanes is served 16 lanes at a time, 8 of one lg and the other 8 n of the
@@ -663,7 +741,7 @@ template <int D> struct StageLds {
     FQ_DEV static int v_at(int lg, int row, int jb) { return lg * VPL + row * VROW + 16 * (jb ^ ((row >> 2) & 3)); }
 };
 
-template <int D, int BITS, typename MT, int KG>
+template <int D, int BITS, typename MT, int KG, bool SEVERAL>
 __global__ __launch_bounds__(64 * tile_waves(KG)) __attribute__((amdgpu_waves_per_eu(tile_waves(KG) / 4, tile_waves(KG) / 4)))
 void shared_tile_kernel(SharedParams a) {
     constexpr int kTW = tile_waves(KG), QB = 16 / kTW, NS = D / 32, NT = D / 16, VC = D / 16;
@@ -679,6 +757,7 @@ void shared_tile_kernel(SharedParams a) {
     __shared__ __attribute__((aligned(16))) uint8_t s_v[2][Lds::VB];
     // metadata as fp16, scales with the codes' factor: [stage & 1][page] [scale, minimum] of K's
     // channels in operand order, and of V's tokens by channel group
+    __shared__ __attribute__((aligned(16))) uint16_t s_bad[2][2][kPg];       // spoil_rows' masks of a stage
     __shared__ __attribute__((aligned(16))) uint16_t s_km[2][2][2][D], s_vm[2][2][4][2][kPg];
     const int tid = threadIdx.x, L = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_id());
     const int n = L & 15, lg = L >> 4;
@@ -693,6 +772,7 @@ void shared_tile_kernel(SharedParams a) {
     const int wg_row0 = tile * RT, row0 = wg_row0 + (w % RG) * (16 * QB);
 
     const bool wave_on = row0 < P.rows;
+    const bool several = SEVERAL && pi == 1;     // rows of several query tokens
 
     int hi[QB], lo = 0, hi_all = P.keys - 1;
     float rs[QB];
@@ -819,10 +899,24 @@ void shared_tile_kernel(SharedParams a) {
             }
         }
     };
+    auto put_bad = [&](int buf, u32x2 b) __attribute__((always_inline)) {      // of any of a token's 16 threads
+        uint32_t any[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            any[j] = (uint32_t)(__builtin_amdgcn_ballot_w64((b[j >> 1] >> (16 * (j & 1)) & 1u) != 0) >> (L & 48)) & 0xFFFFu ? 0xFFFFu : 0u;
+        if (vc == 0) *(u32x2*)&s_bad[buf][pg][4 * vq] = u32x2{any[0] | any[1] << 16, any[2] | any[3] << 16};
+    };
     auto write_v = [&](const Raw& r, int t) __attribute__((always_inline)) {
         const int page = 2 * t + pg, buf = t & 1;
         if (page < code_pages) {
-            const u32x2 sv = *(const u32x2*)&s_vm[buf][pg][vg][0][4 * vq], mv = *(const u32x2*)&s_vm[buf][pg][vg][1][4 * vq];
+            u32x2 sv = *(const u32x2*)&s_vm[buf][pg][vg][0][4 * vq], mv = *(const u32x2*)&s_vm[buf][pg][vg][1][4 * vq];
+            if (several) {
+                asm volatile("");
+                const u32x2 b = {not_finite(sv.x, mv.x), not_finite(sv.y, mv.y)};
+                sv = u32x2{sv.x & ~b.x, sv.y & ~b.y};
+                mv = u32x2{mv.x & ~b.x, mv.y & ~b.y};
+                put_bad(buf, b);
+            }
 #pragma unroll
             for (int i = 0; i < VC; ++i) {
                 const int d = BITS == 8 ? i >> 2 : 0;
@@ -843,6 +937,17 @@ void shared_tile_kernel(SharedParams a) {
 #pragma unroll
                     for (int k = 0; k < VC / 2; ++k) x[j][k] = p[k];
                 }
+            }
+            if (several) {
+                asm volatile("");
+                uint32_t b[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    b[j] = tail_not_finite(x[j]) ? 0xFFFFu : 0u;
+#pragma unroll
+                    for (int k = 0; k < VC / 2; ++k) x[j][k] = b[j] ? 0u : x[j][k];
+                }
+                put_bad(buf, u32x2{b[0] | b[1] << 16, b[2] | b[3] << 16});
             }
 #pragma unroll
             for (int i = 0; i < VC; ++i)
@@ -929,6 +1034,13 @@ void shared_tile_kernel(SharedParams a) {
                     __builtin_amdgcn_sched_barrier(0);
                     pv(s_v[buf], k0 + kPg * u, pb);
                     __builtin_amdgcn_sched_barrier(0);
+                    if (several) {
+                        asm volatile("");
+                        u32x2 bad[4];
+#pragma unroll
+                        for (int T = 0; T < 4; ++T) bad[T] = *(const u32x2*)&s_bad[buf][(k0 + kPg * u) / kPg][16 * T + 4 * lg];
+                        spoil_rows(bad, pb, o);
+                    }
                 }
             }
             if (!UP && t + 1 < t_end) write(t + 1);
@@ -1187,7 +1299,7 @@ hipError_t launch_shared_prefix(const Int4Cache& pc, const TailArgs& pt, const I
     auto attend = [&](int first, int last, int kg) {
         a.first = first; a.last = last;
         const dim3 grid((first == 0 ? a.p[0].wgs : 0) + (last == 1 ? a.p[1].wgs : 0));
-        const bool bf = pc.meta_dtype == FQ_BF16;
+        const bool bf = pc.meta_dtype == FQ_BF16, sev = a.Sq > 1 && last == 1;
 #define FQ_SP(D_, B_)                                                                                                  \
     if (pc.D == D_ && pc.bits == B_ && kg == 0) {                                                                      \
         if (bf) hipLaunchKernelGGL((shared_attn_kernel<D_, B_, bf16>), grid, dim3(64 * kW), 0, st, a);                 \
@@ -1196,8 +1308,10 @@ hipError_t launch_shared_prefix(const Int4Cache& pc, const TailArgs& pt, const I
     }
 #define FQ_ST(D_, B_, K_)                                                                                              \
     if (pc.D == D_ && pc.bits == B_ && kg == K_) {                                                                     \
-        if (bf) hipLaunchKernelGGL((shared_tile_kernel<D_, B_, bf16, K_>), grid, dim3(64 * tile_waves(K_)), 0, st, a);            \
-        else hipLaunchKernelGGL((shared_tile_kernel<D_, B_, f16, K_>), grid, dim3(64 * tile_waves(K_)), 0, st, a);                \
+        if (bf && !sev) hipLaunchKernelGGL((shared_tile_kernel<D_, B_, bf16, K_, false>), grid, dim3(64 * tile_waves(K_)), 0, st, a); \
+        else if (!sev) hipLaunchKernelGGL((shared_tile_kernel<D_, B_, f16, K_, false>), grid, dim3(64 * tile_waves(K_)), 0, st, a);   \
+        else if (bf) hipLaunchKernelGGL((shared_tile_kernel<D_, B_, bf16, K_, true>), grid, dim3(64 * tile_waves(K_)), 0, st, a);     \
+        else hipLaunchKernelGGL((shared_tile_kernel<D_, B_, f16, K_, true>), grid, dim3(64 * tile_waves(K_)), 0, st, a);              \
         return hipGetLastError();                                                                                      \
     }
 #define FQ_SPQ(D_, B_) FQ_SP(D_, B_) FQ_ST(D_, B_, 1) FQ_ST(D_, B_, 2)

@@ -61,7 +61,9 @@ def shared_prefix_attention(q: torch.Tensor, prefix: dict, suffix: dict, *, page
     device, values outside 0 .. S_suffix count as the nearest).  A query with padding alone attends the prefix.
 
     Positions: the suffix's first token follows the prefix's last; the caches hold keys that are rotated already
-    (PagedKVCache.update_rotated).  INT4 and INT8 caches with 64-token pages and head_dim 64 or 128.
+    (PagedKVCache.update_rotated).  A value that is not finite reaches only the queries that attend it, whose outputs
+    are then not finite; in a key it reaches all that attend its page, as the page's scales do.  INT4 and INT8 caches
+    with 64-token pages and head_dim 64 or 128, at most 2^21 query rows (B H_q S_q).
     Returns O (B, H_q, S_q, D) in q's type, with return_lse also the natural-log sum of exponentials (B, H_q, S_q)
     fp32.
     """

@@ -114,6 +114,7 @@ def changed(x, **kw):
     (L.FQ_ERR_INVALID, lambda p, pt, s, st, q: (p, pt, s, st, changed(q, S_q=0))),
     (L.FQ_ERR_INVALID, lambda p, pt, s, st, q: (p, pt, s, st, changed(q, S_q=200))),
     (L.FQ_ERR_UNSUPPORTED, lambda p, pt, s, st, q: (p, pt, s, st, changed(q, H_q=1 << 24))),
+    (L.FQ_ERR_UNSUPPORTED, lambda p, pt, s, st, q: (p, pt, s, st, changed(q, H_q=(1 << 21) // 3 + 2))),     # 2^21 rows at most
     (L.FQ_ERR_UNSUPPORTED, lambda p, pt, s, st, q: (p, pt, s, st, changed(q, dtype=L.FQ_F32))),
     (L.FQ_ERR_UNSUPPORTED, lambda p, pt, s, st, q: (p, pt, s, st, changed(q, q=AT + 8))),
     (L.FQ_ERR_UNSUPPORTED, lambda p, pt, s, st, q: (p, pt, s, st, changed(q, o_strides=L.I64x4(512, 128, 130, 1)))),

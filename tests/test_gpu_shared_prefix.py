@@ -124,6 +124,74 @@ def test_several_tokens(bits, D, B, Hq, H, n, prefix, suffix):
     check(q, p.get_views(0), s.get_views(0), bits)
 
 
+# enough rows for the row tiles in LDS, of 256 and of 128 rows, for both parts and for the prefix alone: pages that
+# fill half a stage, no whole page in either part, rows that end inside a tile, splits
+MANY = [(9, 48, 2, 100, 65, 100), (9, 48, 2, 100, 40, 100), (9, 32, 2, 63, 1823, 63), (9, 32, 2, 63, 95, 64),
+        (9, 32, 2, 63, 65, 63), (9, 48, 2, 33, 40, 33), (5, 24, 1, 100, 4415, 140), (3, 24, 2, 60, 6011, 60),
+        (4, 40, 1, 160, 2000, 1000)]
+
+
+@pytest.mark.parametrize("bits,D,dtype,kw", [
+    (4, 128, torch.bfloat16, {}),
+    (4, 128, torch.float16, dict(meta_dtype=torch.float16, v_group=32)),
+    (4, 64, torch.float16, dict(v_group=32)),
+    (8, 128, torch.bfloat16, dict(meta_dtype=torch.float16)),
+    (8, 64, torch.bfloat16, {}),
+])
+@pytest.mark.parametrize("B,Hq,H,n,prefix,suffix", MANY)
+def test_many_rows(bits, D, dtype, kw, B, Hq, H, n, prefix, suffix):
+    gen = torch.Generator(device=DEV).manual_seed(n + prefix + suffix)
+    p, s = filled(bits, gen, 1, H, D, prefix, **kw), filled(bits, gen, B, H, D, suffix, **kw)
+    q = torch.randn(B, Hq, n, D, device=DEV, generator=gen).to(dtype)
+    check(q, p.get_views(0), s.get_views(0), bits)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("n,suffix", [(100, 260), (37, 199)])
+def test_many_rows_with_left_padding(bits, n, suffix):
+    """Starts as in test_left_padding, among them ones that leave a query token none of its own keys."""
+    gen = torch.Generator(device=DEV).manual_seed(7 + n)
+    starts = torch.tensor([0, 1, 63, 64, 65, 128, suffix - n + 2, suffix, 1000, -5], dtype=torch.int32, device=DEV)
+    B = len(starts)
+    p = filled(bits, gen, 1, 2, 128, 130)
+    s = CLASSES[bits](batch_size=B, num_layers=1, num_kv_heads=2, head_dim=128, max_seq_len=320, device=DEV)
+    k, v = (torch.randn(B, 2, suffix, 128, device=DEV, generator=gen).to(torch.bfloat16) for _ in range(2))
+    for b, x in enumerate(starts.tolist()):
+        v[b, :, 0:max(0, min(x, suffix)):2] = float("nan")
+        v[b, :, 1:max(0, min(x, suffix)):2] = float("inf")
+    s.update_quantized(k, v, 0)
+    q = torch.randn(B, 48, n, 128, device=DEV, generator=gen).to(torch.bfloat16)
+    check(q, p.get_views(0), s.get_views(0), bits, suffix_start=starts)
+
+
+@pytest.mark.parametrize("bits,D,kw", [(4, 128, {}), (4, 128, dict(v_group=32)), (4, 64, {}), (8, 128, {}), (8, 64, {})])
+@pytest.mark.parametrize("B,Hq,H,n,prefix,suffix", [(3, 6, 2, 5, 100, 70), (2, 4, 2, 70, 65, 140), (9, 32, 2, 63, 95, 64),
+                                                    (9, 48, 2, 100, 65, 128), (9, 48, 2, 100, 65, 100)])
+def test_a_value_that_is_not_finite_stays_with_the_queries_that_attend_it(bits, D, kw, B, Hq, H, n, prefix, suffix):
+    """NaN and infinities among the values of a step's own tokens, in whole pages and in the partial one, one sequence
+    without: queries before the first of them are as without it, queries behind it are not finite."""
+    gen = torch.Generator(device=DEV).manual_seed(n + suffix)
+    p = filled(bits, gen, 1, H, D, prefix, **kw)
+    k, v = (torch.randn(B, H, suffix, D, device=DEV, generator=gen).to(torch.bfloat16) for _ in range(2))
+    first = torch.randint(suffix - n + 1, suffix, (B,), device=DEV, generator=gen)
+    first[0], first[1], first[-1] = suffix - 1, suffix - n + 1, suffix       # the last query alone; all but one; none
+    bad = v.clone()
+    for b in range(B - 1):
+        bad[b, :, first[b]] = (float("nan"), float("inf"), -float("inf"))[b % 3]
+    q = torch.randn(B, Hq, n, D, device=DEV, generator=gen).to(torch.bfloat16)
+    outs = []
+    for x in (v, bad):
+        s = CLASSES[bits](batch_size=B, num_layers=1, num_kv_heads=H, head_dim=D, max_seq_len=suffix + 64, device=DEV, **kw)
+        s.update_quantized(k, x, 0)
+        outs.append(shared_prefix_attention(q, p.get_views(0), s.get_views(0), return_lse=True))
+    (want, wl), (got, gl) = outs
+    before = torch.arange(n, device=DEV) + suffix - n < first[:, None]
+    assert bool(before.any()) and not bool(before.all())
+    assert torch.equal(got.transpose(1, 2)[before], want.transpose(1, 2)[before])
+    assert torch.equal(gl, wl)
+    assert not bool(got.transpose(1, 2)[~before].isfinite().any())
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("n", [1, 5])
 def test_left_padding(bits, n):
