@@ -347,7 +347,8 @@ constexpr int attn_waves(int d) { return d == 64 ? 3 : 2; }      // a SIMD, as t
 // operands its own, and the four waves' states meet in LDS.  The next page's metadata, keys and
 // values are loaded into the registers of this one's as each has been used: a second set would
 // leave room for one wave a SIMD instead of two (the suffixes of 64 sequences, INT8: 24 us then,
-// 13.5 now; three or four waves a SIMD spill and are slower).
+// 13.5 now; three or four waves a SIMD spill and are slower).  128 suffixes of 640 tokens of 8 KV
+// heads in INT4: 27 us for 92 MB (3.4 TB/s), half of it waits for a page, half vector issue.
 template <int D, int BITS, typename MT>
 __global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(attn_waves(D), attn_waves(D))))
 void shared_attn_kernel(SharedParams a) {
@@ -706,6 +707,13 @@ void shared_attn_kernel(SharedParams a) {
 // and the upper ones V; a read feeds one (1.9 ns of LDS to 1.8 of the four matrix cores), but three
 // other waves have work while one waits.  512 rows over 32768 tokens in INT4: 102 us with 8 waves for
 // KG = 1, 106 with 16; 128 rows: 49 with 8 for KG = 2, 47 with 16; 320 rows over 16384: 60 and 49.
+//
+// 4 x 512 rows over 16411 tokens of 8 KV heads in INT8: 151 us, 0.92 PFLOP/s (a large fp16 product
+// reaches 1.17).  A matrix instruction takes 7.1 ns of a SIMD and hides two vector instructions of the
+// other wave; each further one adds 2.3 ns.  Left out one at a time, the products were 63 %, scores to
+// weights 20 % and the operands' making 16 % of the time: hardly any overlap.  Keeping the two waves of
+// a SIMD in different parts by barriers did not bring it (a part then lasts as long as one wave's
+// serial instructions).
 //
 // SEVERAL: a launch with suffixes of several query tokens (spoil_rows); without it a step of one token
 // is 1 to 2 % faster.
@@ -1119,7 +1127,7 @@ void shared_tile_kernel(SharedParams a) {
     }
 }
 
-// Joins the shares of a row: prefix splits, then suffix splits.  D/4 lanes take four channels
+// Joins the shares of a row: prefix splits, then suffix splits; 33 MB of shares in 9.5 us (3.5 TB/s).  D/4 lanes take four channels
 // each of every MG-th share (its loads all go out before the first is used: the kernel is
 // little but the latency of reading the shares), and the MG groups meet in LDS, in order.
 template <int D, int MG>

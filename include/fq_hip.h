@@ -630,8 +630,10 @@ typedef struct fq_shared_query {
  * each with S completed tokens (whole 64-token pages, may be 0) and the bf16 rows of its partial
  * page (tail NULL or len 0: none).  At least one prefix token and S_q suffix tokens.  D is 64 or
  * 128; the two caches have one metadata type.  K code rows are 16-byte aligned (INT4 with
- * D == 64: 8).  K values up to 2e6 and V values up to 3e4 in size.  Two or three launches;
- * every byte of the workspace is written before it is read.  Deterministic. */
+ * D == 64: 8).  K values up to 2e6 and V values up to 3e4 in size;
+ * with S_q > 1 the outputs of queries that attend a value that is not finite are not finite, the
+ * others' as without it.  At most 2^21 query rows (B H_q S_q).  Two or three launches; every byte of
+ * the workspace is written before it is read.  Deterministic. */
 int fq_shared_prefix_int4(const fq_int4_cache* prefix, const fq_tail* prefix_tail,
                           const fq_int4_cache* suffix, const fq_tail* suffix_tail, const fq_shared_query* query,
                           void* workspace, size_t workspace_bytes, fq_stream_t stream);
