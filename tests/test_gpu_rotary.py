@@ -209,6 +209,39 @@ def test_dequantize_cache(bits, D, kw, length, start):
         assert torch.equal(gk, K) and torch.equal(gv, V)
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+def test_offsets_past_32_bits(bits):
+    """Heads of the cache, and of q, k and v, more than 2^32 bytes apart."""
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    room = torch.empty(5 << 30, dtype=torch.uint8, device=DEV)
+    at = [0]
+
+    def far(t):
+        size, st = t.element_size(), list(t.contiguous().stride())
+        st[0], st[1] = (1 << 24) // size, ((1 << 32) + (1 << 12)) // size     # a batch's row holds all tensors, 2^18 apart
+        x = room.view(t.dtype).as_strided(t.shape, st, at[0] // size)
+        at[0] += 1 << 18
+        x.copy_(t)
+        return x
+
+    c = make_cache(bits)
+    buffers = {n: t.clone() for n, t in c.buffers(0).items()}
+    spread = {n: far(t) for n, t in buffers.items()}
+    seen = 0
+    for n in (70, 1, 130):
+        q, k, v = (tokens(gen, 2, 2, n, 128) for _ in range(3))
+        cos, sin = angles(2, seen + torch.arange(n, device=DEV), 128, torch.float32, gen)
+        want = rotate_append(q, k, v, cos, sin, buffers, seen)
+        got = rotate_append(far(q), far(k), far(v), cos, sin, spread, seen)
+        assert torch.equal(got, want)
+        seen += n
+        for name, t in buffers.items():
+            assert torch.equal(spread[name], t), name
+        gk, gv = dequantize_cache(spread, seen)
+        wk, wv = dequantize_cache(buffers, seen)
+        assert torch.equal(gk, wk) and torch.equal(gv, wv)
+
+
 @pytest.mark.parametrize("bits", [4, 8, 3])
 def test_a_prompt_and_decode_steps(bits):
     """A layer as a model runs it: the prompt rotated into the cache and attended, then steps of one token."""

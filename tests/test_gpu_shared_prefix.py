@@ -192,6 +192,32 @@ def test_a_value_that_is_not_finite_stays_with_the_queries_that_attend_it(bits, 
     assert not bool(got.transpose(1, 2)[~before].isfinite().any())
 
 
+def far_apart(views):
+    """The views' tensors with their heads more than 2^32 bytes apart, as slices of a long cache have them."""
+    room = torch.empty((5 << 30), dtype=torch.uint8, device=DEV)
+    out, at = dict(views), 0
+    for name, t in views.items():
+        if not torch.is_tensor(t) or t.numel() == 0:
+            continue
+        size = t.element_size()
+        st = list(t.contiguous().stride())
+        st[0], st[1] = (1 << 22) // size, ((1 << 32) + (1 << 12)) // size
+        out[name] = room.view(t.dtype).as_strided(t.shape, st, at // size)
+        out[name].copy_(t)
+        at += 1 << 18
+    return out
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("B,Hq,n,prefix,suffix", [(3, 6, 1, 150, 70), (9, 32, 63, 95, 70)])
+def test_offsets_past_32_bits(bits, B, Hq, n, prefix, suffix):
+    gen = torch.Generator(device=DEV).manual_seed(29)
+    p, s = filled(bits, gen, 1, 2, 128, prefix), filled(bits, gen, B, 2, 128, suffix)
+    q = torch.randn(B, Hq, n, 128, device=DEV, generator=gen).to(torch.bfloat16)
+    want = shared_prefix_attention(q, p.get_views(0), s.get_views(0))
+    assert torch.equal(shared_prefix_attention(q, far_apart(p.get_views(0)), far_apart(s.get_views(0))), want)
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("n", [1, 5])
 def test_left_padding(bits, n):
