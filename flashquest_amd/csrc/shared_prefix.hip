@@ -31,8 +31,9 @@
 // weights: beyond two vector instructions a matrix instruction each further one adds its own
 // four cycles, so they have to be few of each page.
 //
-// Operands are fp16, whose 11 bits leave errors below those of 16-bit outputs (bf16's 8 do
-// not): q exact after a power of two per row (16-bit inputs), K and V one rounding of
+// Operands are fp16: errors of 4e-4 of the outputs' size, an fp16 output's own rounding (2e-4)
+// included; a bf16 output's is 1.7e-3.  (bf16 operands, with 8 bits for 11, would leave eight times
+// as much.)  q is exact after a power of two per row (16-bit inputs), K and V one rounding of
 // code * scale + min, K times 2^-6 (|K| up to 2e6 stays finite, |V| up to 3e4; K is exact to
 // 2^-19, V to 2^-25, where they are small), P times 2^7 (exact to 2^-32 of a row's largest
 // weight where it is small).  Sums, maxima and outputs are fp32.
